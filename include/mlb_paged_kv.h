@@ -41,7 +41,8 @@ enum {
   MLB_DEV_SLOT_RANGE = 1,   /* slot_mapping entry outside [0, num_blocks * block_size): row not written */
   MLB_DEV_BLOCK_RANGE = 2,  /* block_tables entry outside [0, num_blocks): page treated as empty        */
   MLB_DEV_WAIT_TIMEOUT = 4, /* a bounded wait on a page copy gave up: output of that unit is invalid    */
-  MLB_DEV_COPY_RANGE = 8    /* block-copy pair outside [0, num_blocks): pair skipped                    */
+  MLB_DEV_COPY_RANGE = 8,   /* block-copy pair outside [0, num_blocks): pair skipped                    */
+  MLB_DEV_POSITION_RANGE = 16 /* position outside the rotation table: row not written                   */
 };
 
 /* Description of the last failing call on this thread ("" if none). */
@@ -383,6 +384,83 @@ MLB_API int mlb_splitk_reduce_exchange(const float* partial_o, const float* part
                       int64_t out_stride_tok, int64_t out_stride_head, void* const* packets,
                       int64_t packet_capacity, int rank, int world, uint32_t* state, int64_t timeout_ns,
                       int32_t* err_word, void* stream);
+
+/*
+ * 4-bit pools.  uint8 [num_blocks, num_kv_heads, 17, head_dim / 2], contiguous, 16 tokens a block (the block ids,
+ * tables and slots of the 16-bit pools): rows 0..15 of a (block, head) are its tokens' codes, two e2m1 values a
+ * byte (dim 2i in the low nibble); row 16 holds one scale byte for each run of 32 dims of a token, at
+ * [run][2 * (token % 8) + token / 8].  A scale byte b is the fp16 with bits b << 7; a stored value is code * scale.
+ * head_dim 64, 128 or 256.  mlb_block_copy moves such blocks as any others (block_bytes = num_kv_heads * 17 *
+ * head_dim / 2).  No reference counterpart: the reference's pools are 16- or 32-bit.
+ */
+
+/*
+ * kv_append into 4-bit pools: row (token i, head h) of k and v is stored at slot slot_mapping[i].  For each run of
+ * 32 dims, scale = max|x| / 6 rounded to the byte format (nearest, ties to even, at most 10240) and code = x / scale
+ * rounded to e2m1 (nearest, ties to even); both roundings see the exact quotient.  Magnitudes above 61440 are
+ * stored as 61440, NaN as 0; a run whose largest magnitude is below 6 * 2^-18 is stored as zeros.  Slots must be
+ * distinct; a slot out of range is skipped and flagged (MLB_DEV_SLOT_RANGE).  Other arguments as mlb_kv_append.
+ */
+MLB_API int mlb_kv_append_fp4(void* k_cache, void* v_cache, int64_t num_blocks, const int64_t* slot_mapping,
+                      const void* k, int64_t k_stride_tok, int64_t k_stride_head, const void* v,
+                      int64_t v_stride_tok, int64_t v_stride_head, int in_dtype, int64_t num_tokens,
+                      int num_kv_heads, int head_dim, int32_t* err_word, void* stream);
+
+/*
+ * The values that 4-bit pools hold at slot_mapping, as rows k_out / v_out [num_tokens, num_kv_heads, head_dim]
+ * (contiguous, 16-byte aligned) of out_dtype; code * scale is exact in all three.  A slot out of range reads as
+ * zeros and is flagged (MLB_DEV_SLOT_RANGE); the same slot may be read more than once.
+ */
+MLB_API int mlb_kv_read_fp4(const void* k_cache, const void* v_cache, int64_t num_blocks, const int64_t* slot_mapping,
+                      void* k_out, void* v_out, int out_dtype, int64_t num_tokens, int num_kv_heads, int head_dim,
+                      int32_t* err_word, void* stream);
+
+/*
+ * Norm of each query and key head, with the rotation by position in the same pass:
+ *   y = x * rsqrt(mean(x^2) + eps) * weight      (q_weight / k_weight: [head_dim] of dtype; NULL: y = x)
+ *   out[i] = y[i] c - y[i + r/2] s,  out[i + r/2] = y[i + r/2] c + y[i] s   for i < r/2 (r = rot_dim)
+ *   out[i] = y[i]                                                            for i >= r
+ * with c = cos_sin[p][i], s = cos_sin[p][r/2 + i], p = positions[token], in fp32 and rounded once to dtype.
+ * q [num_tokens, num_heads, head_dim] and k [num_tokens, num_kv_heads, head_dim] with strides in elements; cos_sin:
+ * fp32 [num_positions, rot_dim], contiguous; rot_dim a multiple of 16, at most head_dim (0: no rotation); the
+ * table and the weights 16-byte aligned.  q_out / k_out may be q / k themselves (same strides).  A position out of
+ * range leaves the token's rows unwritten and is flagged (MLB_DEV_POSITION_RANGE).  Rotation as the reference's
+ * model applies it before the backend's forward (src/minillm/model/llama.py).
+ */
+MLB_API int mlb_qk_norm_rope(const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k,
+                      int64_t k_stride_tok, int64_t k_stride_head, int dtype, int64_t num_tokens, int num_heads,
+                      int num_kv_heads, int head_dim, const int64_t* positions, const float* cos_sin,
+                      int64_t num_positions, int rot_dim, const void* q_weight, const void* k_weight, float eps,
+                      void* q_out, int64_t q_out_stride_tok, int64_t q_out_stride_head, void* k_out,
+                      int64_t k_out_stride_tok, int64_t k_out_stride_head, int32_t* err_word, void* stream);
+
+/*
+ * mlb_qk_norm_rope followed by mlb_kv_append_fp4 of its keys and of v, as one launch (bit-identical to the two
+ * calls: the keys are rounded to dtype before they are stored).  Needs rot_dim == head_dim.  A position or slot out
+ * of range is flagged; the first leaves all of the token's rows unwritten, the second its cache rows.
+ */
+MLB_API int mlb_qk_norm_rope_append_fp4(const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k,
+                      int64_t k_stride_tok, int64_t k_stride_head, const void* v, int64_t v_stride_tok,
+                      int64_t v_stride_head, int dtype, int64_t num_tokens, int num_heads, int num_kv_heads,
+                      int head_dim, const int64_t* positions, const float* cos_sin, int64_t num_positions,
+                      int rot_dim, const void* q_weight, const void* k_weight, float eps, void* q_out,
+                      int64_t q_out_stride_tok, int64_t q_out_stride_head, void* k_cache, void* v_cache,
+                      int64_t num_blocks, const int64_t* slot_mapping, int32_t* err_word, void* stream);
+
+/*
+ * mlb_paged_attention over 4-bit pools: q and out are fp16 or bf16, the plan is mlb_plan_attention's (units,
+ * shared units and query tiles alike), partial rows are completed by mlb_splitk_reduce.  head_dim 64 / 128 / 256,
+ * at most 8 query heads per KV head, scale positive.  Stored values enter the products exactly; P is rounded to
+ * fp16, sums are fp32.
+ */
+MLB_API int mlb_paged_attention_fp4(const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k_cache,
+                      const void* v_cache, int dtype, int64_t num_blocks, int num_heads, int num_kv_heads,
+                      int head_dim, float scale, const int32_t* block_tables, int64_t bt_stride,
+                      const int32_t* seq_lens, const int32_t* qo_indptr, int num_seqs, const mlb_work_unit* units,
+                      int64_t num_units, const mlb_shared_unit* shared_units, int64_t num_shared_units,
+                      const mlb_share_member* members, float* partial_o, float* partial_lse,
+                      int64_t num_partial_rows, void* out, int64_t out_stride_tok, int64_t out_stride_head,
+                      const mlb_out_targets* out_targets, int32_t* err_word, void* stream);
 
 #ifdef __cplusplus
 }

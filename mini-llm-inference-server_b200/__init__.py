@@ -12,10 +12,12 @@ The directory name is not a Python identifier; import it with
 
 from . import ops
 from .attention import AttentionBackend, AttentionMetadata, B200Backend, DeviceFault, SeqStep, get_backend
-from .cache import BLOCK_SIZE, BlockManager, KVShape, PagedKVCache, PagedStep, PrefixCache
-from .ops import AttentionPlan, Workspace, block_copy, kv_append, paged_attention, plan_attention
+from .cache import BLOCK_SIZE, BlockManager, KVShape, PagedKVCache, PagedKVCacheFP4, PagedStep, PrefixCache
+from .ops import (AttentionPlan, Rotary, Workspace, block_copy, kv_append, kv_append_fp4, kv_read_fp4, paged_attention,
+                  paged_attention_fp4, plan_attention, qk_norm_rope, qk_norm_rope_append_fp4, rotary_table)
 
 __all__ = ["AttentionBackend", "AttentionMetadata", "AttentionPlan", "B200Backend", "BLOCK_SIZE", "BlockManager",
            "DeviceFault",
-           "KVShape", "PagedKVCache", "PagedStep", "PrefixCache", "SeqStep", "Workspace", "block_copy",
-           "get_backend", "kv_append", "ops", "paged_attention", "plan_attention"]
+           "KVShape", "PagedKVCache", "PagedKVCacheFP4", "PagedStep", "PrefixCache", "Rotary", "SeqStep", "Workspace",
+           "block_copy", "get_backend", "kv_append", "kv_append_fp4", "kv_read_fp4", "ops", "paged_attention",
+           "paged_attention_fp4", "plan_attention", "qk_norm_rope", "qk_norm_rope_append_fp4", "rotary_table"]

@@ -16,13 +16,14 @@ LIB_PATH = Path(__file__).with_name("_mlb_paged_kv.so")
 MLB_F32, MLB_F16, MLB_BF16 = 0, 1, 2
 MLB_OK, MLB_EINVAL, MLB_EUNSUPPORTED, MLB_ECUDA, MLB_ENOSPACE = 0, 1, 2, 3, 4
 # bits kernels OR into the device error word
-DEV_SLOT_RANGE, DEV_BLOCK_RANGE, DEV_WAIT_TIMEOUT, DEV_COPY_RANGE = 1, 2, 4, 8
+DEV_SLOT_RANGE, DEV_BLOCK_RANGE, DEV_WAIT_TIMEOUT, DEV_COPY_RANGE, DEV_POSITION_RANGE = 1, 2, 4, 8, 16
 
 EXPORTS = ("mlb_last_error", "mlb_abi_version", "mlb_kv_append", "mlb_plan_attention", "mlb_paged_attention",
            "mlb_splitk_reduce", "mlb_block_copy", "mlb_paged_attention_noalloc", "mlb_ipc_alloc", "mlb_ipc_open",
            "mlb_ipc_close", "mlb_ipc_free", "mlb_peer_barrier", "mlb_set_programmatic_launch",
            "mlb_splitk_reduce_gather", "mlb_set_tensor_core_prefix", "mlb_paged_attention_append",
-           "mlb_build_metadata", "mlb_set_concurrent_prefix", "mlb_splitk_reduce_exchange")
+           "mlb_build_metadata", "mlb_set_concurrent_prefix", "mlb_splitk_reduce_exchange", "mlb_kv_append_fp4",
+           "mlb_kv_read_fp4", "mlb_qk_norm_rope", "mlb_qk_norm_rope_append_fp4", "mlb_paged_attention_fp4")
 ABI_VERSION = 10
 NOALLOC_SCRATCH_BYTES = 8 << 20  # MLB_NOALLOC_SCRATCH_BYTES
 MAX_OUT_DESTS = 8  # MLB_MAX_OUT_DESTS
@@ -111,6 +112,21 @@ _SIGNATURES = {
     "mlb_splitk_reduce_exchange": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_int64, c_int,
                                            c_int, c_int, c_void_p, c_int64, c_int64, POINTER(c_void_p), c_int64,
                                            c_int, c_int, c_void_p, c_int64, c_void_p, c_void_p]),
+    "mlb_kv_append_fp4": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p,
+                                  c_int64, c_int64, c_int, c_int64, c_int, c_int, c_void_p, c_void_p]),
+    "mlb_kv_read_fp4": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int,
+                                c_int, c_void_p, c_void_p]),
+    "mlb_qk_norm_rope": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int, c_int64, c_int, c_int,
+                                 c_int, c_void_p, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_float, c_void_p,
+                                 c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p]),
+    "mlb_qk_norm_rope_append_fp4": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64,
+                                            c_int64, c_int, c_int64, c_int, c_int, c_int, c_void_p, c_void_p, c_int64,
+                                            c_int, c_void_p, c_void_p, c_float, c_void_p, c_int64, c_int64, c_void_p,
+                                            c_void_p, c_int64, c_void_p, c_void_p, c_void_p]),
+    "mlb_paged_attention_fp4": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int, c_int64, c_int, c_int,
+                                        c_int, c_float, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p,
+                                        c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p,
+                                        c_int64, c_int64, POINTER(OutTargets), c_void_p, c_void_p]),
 }
 
 _lib: ctypes.CDLL | None = None

@@ -9,6 +9,9 @@
    attention launch stores the rows and uses them for the pages that hold them;
 3. K2a paged attention over `meta.block_tables_i32` + K2b split-K reduction (replaces paged_attention,
    paged_torch_ref.py:40-74, and FlashInfer's run(), flashinfer_backend.py:46).
+With 4-bit pools (uint8, `PagedKVCacheFP4`) the same three steps run on the 4-bit kernels: `kv_append_fp4`, paged
+attention over the codes, the reduction.  `rotary` puts the norm and rotation of queries and keys in front, in the
+append's launch where that is one (4-bit pools, whole heads rotated).
 No host synchronisation happens inside `forward` with this package's `AttentionMetadata`; every launch goes
 on torch's current stream.  With the reference's own metadata object (only the reference's fields), the
 first layer of a step copies its block tables and slot_mapping back to the host once (`host_view`), so the
@@ -25,8 +28,10 @@ import torch
 import torch.nn.functional as F
 
 from .. import _lib
-from ..ops import (AttentionPlan, Workspace, attention_partials, can_fuse_append, kv_append, paged_attention,
-                   plan_attention, splitk_reduce_exchange, splitk_reduce_gather)
+from ..ops import (BLOCK_SIZE, AttentionPlan, Rotary, Workspace, attention_partials, attention_partials_fp4,
+                   can_fuse_append, is_fp4, kv_append, kv_append_fp4, paged_attention, paged_attention_fp4,
+                   plan_attention, pool_kv_heads, qk_norm_rope, qk_norm_rope_append_fp4, splitk_reduce_exchange,
+                   splitk_reduce_gather)
 from .base import AttentionBackend
 from .metadata import host_view
 
@@ -102,30 +107,47 @@ class B200Backend(AttentionBackend):
             tables = self.host_fields(meta)[0] if dtype != torch.float32 else None
             self._plan = plan_attention(meta.query_start_loc, meta.seq_lens, meta.block_tables_i32.shape[1],
                                         num_heads, num_kv_heads, device, meta.block_size, self.num_sms,
-                                        self.pages_per_unit, block_tables_host=tables)
+                                        self.pages_per_unit, block_tables_host=tables, pool_dtype=dtype)
             self._planned, self._plan_key = meta, key
         return self._plan
 
-    def forward(self, q, k, v, k_cache, v_cache, meta, out_targets=None, peer_gather=None):
+    def forward(self, q, k, v, k_cache, v_cache, meta, out_targets=None, peer_gather=None,
+                rotary: Rotary | None = None):
         """out_targets (optional, `ops.out_targets`): store the output rows there and return None.
         peer_gather (optional, `(PeerOutputs, slot, head_offset)`, used by KV-head sharding): put every row
         in every rank's gathered buffer of that slot (the reduction carries the all-gather: as flagged
-        packets, or plain stores followed by the peers' barrier, as the PeerOutputs was built)."""
-        if k_cache.shape[1] != meta.block_size:
-            raise ValueError(f"pool block size {k_cache.shape[1]} != metadata block size {meta.block_size}")
+        packets, or plain stores followed by the peers' barrier, as the PeerOutputs was built).
+        rotary (optional, `ops.Rotary`): q and k come from the projection; norm and rotate them at
+        meta.positions first."""
+        fp4 = is_fp4(k_cache)
+        pool_block = BLOCK_SIZE if fp4 else k_cache.shape[1]
+        if pool_block != meta.block_size:
+            raise ValueError(f"pool block size {pool_block} != metadata block size {meta.block_size}")
         err = self._error_word(q.device) if self.check_errors else None
-        plan = self.plan(meta, q.shape[1], k_cache.shape[2], q.device, k_cache.dtype)
+        plan = self.plan(meta, q.shape[1], pool_kv_heads(k_cache), q.device, k_cache.dtype)
         append = None
-        if self.fuse_append and can_fuse_append(plan, k_cache, k, v) and self.host_fields(meta)[1]:
+        if rotary is not None and not (fp4 and rotary.cos_sin.shape[1] == q.shape[2]):
+            q, k = qk_norm_rope(q, k, meta.positions, rotary.cos_sin, rotary.q_weight, rotary.k_weight, rotary.eps,
+                                err=err)
+            rotary = None
+        if fp4 and rotary is not None:
+            q = qk_norm_rope_append_fp4(q, k, v, meta.positions, rotary.cos_sin, k_cache, v_cache, meta.slot_mapping,
+                                        rotary.q_weight, rotary.k_weight, rotary.eps, err=err)
+        elif fp4:
+            kv_append_fp4(k_cache, v_cache, meta.slot_mapping, k, v, err)
+        elif self.fuse_append and can_fuse_append(plan, k_cache, k, v) and self.host_fields(meta)[1]:
             append = (k, v, meta.slot_mapping)
         else:
             kv_append(k_cache, v_cache, meta.slot_mapping, k, v, err)
         self.last_append_fused = append is not None
         if peer_gather is not None:
             peers, slot, head_offset = peer_gather
-            attention_partials(q, k_cache, v_cache, meta.block_tables_i32, meta.seq_lens_i32, meta.qo_indptr, plan,
-                               self._workspace, err=err, targets=peers.local_targets(slot, head_offset),
-                               append=append)
+            args = (q, k_cache, v_cache, meta.block_tables_i32, meta.seq_lens_i32, meta.qo_indptr, plan, self._workspace)
+            local = peers.local_targets(slot, head_offset)
+            if fp4:
+                attention_partials_fp4(*args, err=err, targets=local)
+            else:
+                attention_partials(*args, err=err, targets=local, append=append)
             if peers.use_packets(q.shape[0]):
                 splitk_reduce_exchange(plan, self._workspace, peers, slot, q.dtype, q.shape[2], q.device)
             else:
@@ -133,6 +155,9 @@ class B200Backend(AttentionBackend):
                                      q.dtype, q.shape[2], q.device)
                 peers.barrier()
             out = None
+        elif fp4:
+            out = paged_attention_fp4(q, k_cache, v_cache, meta.block_tables_i32, meta.seq_lens_i32, meta.qo_indptr,
+                                      plan, self._workspace, err=err, targets=out_targets)
         else:
             out = paged_attention(q, k_cache, v_cache, meta.block_tables_i32, meta.seq_lens_i32, meta.qo_indptr,
                                   plan, self._workspace, err=err, targets=out_targets, append=append)
@@ -155,5 +180,6 @@ class B200Backend(AttentionBackend):
             names = [n for b, n in ((_lib.DEV_SLOT_RANGE, "slot out of range"),
                                     (_lib.DEV_BLOCK_RANGE, "block id out of range"),
                                     (_lib.DEV_WAIT_TIMEOUT, "page copy wait timed out"),
-                                    (_lib.DEV_COPY_RANGE, "block-copy pair out of range")) if bits & b]
+                                    (_lib.DEV_COPY_RANGE, "block-copy pair out of range"),
+                                    (_lib.DEV_POSITION_RANGE, "position outside the rotation table")) if bits & b]
             raise DeviceFault("device fault flags: " + ", ".join(names))

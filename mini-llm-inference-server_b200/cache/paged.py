@@ -69,6 +69,38 @@ class PagedKVCache:
         ops.block_copy(self._ptrs, self.k[0], s, d, err)
 
 
+class PagedKVCacheFP4(PagedKVCache):
+    """`PagedKVCache` with 4-bit pools: uint8 [num_blocks, Hkv, 17, Dh / 2] per layer (16 tokens' e2m1 codes and a
+    row of scales, include/mlb_paged_kv.h), 0.266 of the 16-bit pool's bytes, so a budget holds 3.76 times the
+    tokens.  Same block ids, tables, copy-on-write and compaction; `B200Backend.forward` takes its `.k` / `.v`."""
+
+    def __init__(self, config, num_blocks: int, device: torch.device | str) -> None:
+        shape = ops.fp4_pool_shape(num_blocks, config.num_key_value_heads, config.head_dim)
+        self.storage = torch.zeros((2, config.num_hidden_layers, *shape), device=device, dtype=torch.uint8)
+        self.k = list(self.storage[0].unbind(0))
+        self.v = list(self.storage[1].unbind(0))
+        self.num_blocks = num_blocks
+        self.block_size = BLOCK_SIZE
+        self._ptrs: torch.Tensor | None = None
+
+    @staticmethod
+    def bytes_per_block(config, dtype: torch.dtype = torch.uint8, block_size: int = BLOCK_SIZE) -> int:
+        if dtype is not torch.uint8 or block_size != BLOCK_SIZE:
+            raise ValueError(f"4-bit pools are uint8 with {BLOCK_SIZE} tokens a block, got {dtype}, {block_size}")
+        _, heads, rows, half = ops.fp4_pool_shape(1, config.num_key_value_heads, config.head_dim)
+        return 2 * config.num_hidden_layers * heads * rows * half
+
+    @classmethod
+    def blocks_for_bytes(cls, config, dtype: torch.dtype, num_bytes: int, block_size: int = BLOCK_SIZE) -> int:
+        return num_bytes // cls.bytes_per_block(config, dtype, block_size)
+
+    def read(self, layer: int, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16,
+             err: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+        """The (k, v) rows [N, Hkv, Dh] that a layer holds at `slots` (device int64), as values: what a move to
+        another pool type or a contiguous attention path needs."""
+        return ops.kv_read_fp4(self.k[layer], self.v[layer], slots, dtype, err)
+
+
 class PagedStep:
     """What the reference's model asks of a KV cache during one ragged step (cache/paged.py:48-69).  The
     backend's `forward` writes and reads the pool itself and the engine counts each request's cached tokens,

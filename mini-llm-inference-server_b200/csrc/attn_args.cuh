@@ -27,6 +27,7 @@ struct AttnArgs {
   int64_t part_rows;  // rows of part_o / part_lse (writes beyond are skipped and flagged)
   mlb_out_targets out;  // final rows: one or more destinations (the call's `out`, or every rank's buffer)
   int out_vec;          // out_vec_ok(out): rows may be stored with packed 16-byte-aligned stores
+  int q_vec;            // 4-bit pools: q rows start 16-byte aligned (packed loads)
   int32_t* err;
   // fused append (mlb_paged_attention_append), app_k == nullptr otherwise: the step's new rows, taken from
   // here for every page that holds them and stored into the pools at app_slots by the row's last query tile

@@ -10,6 +10,7 @@
 #include <vector>
 
 #include "attn_args.cuh"
+#include "row_args.cuh"
 
 namespace mlb {
 cudaError_t launch_kv_append(void* k_cache, void* v_cache, int cache_dtype, int64_t num_slots, const int64_t* slots,
@@ -33,6 +34,11 @@ cudaError_t launch_splitk_reduce_exchange(const float* po, const float* plse, co
                                           void* out, int64_t out_st, int64_t out_sh, void* const* packets, int rank,
                                           int world, uint32_t* state, int64_t timeout_ns, int32_t* err, int num_sms,
                                           cudaStream_t s);
+cudaError_t launch_norm_rope(const RowArgs& a, int dtype, int dh, bool append, int num_sms, cudaStream_t s);
+cudaError_t launch_fp4_append(const RowArgs& a, int dtype, int dh, int num_sms, cudaStream_t s);
+cudaError_t launch_fp4_read(const RowArgs& a, int dtype, int dh, int num_sms, cudaStream_t s);
+cudaError_t launch_fp4_attention(const AttnArgs& a, int dtype, int dh, int64_t num_units, cudaStream_t s);
+cudaError_t launch_fp4_shared(const AttnArgs& a, int dtype, int dh, int64_t num_units, cudaStream_t s);
 cudaError_t launch_block_copy(void* const* pools, int num_pools, int64_t num_blocks, int64_t block_bytes,
                               const int32_t* src, const int32_t* dst, int64_t num_pairs, int32_t* err, int num_sms,
                               cudaStream_t s);
@@ -789,6 +795,201 @@ int mlb_build_metadata(const int64_t* in, int64_t num_ids, int num_seqs, int64_t
   return cuda_status(mlb::launch_build_metadata(in, num_ids, num_seqs, num_tokens, num_pages, width, block_size, out64,
                                                 out32, static_cast<cudaStream_t>(stream)),
                      "build_metadata launch");
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------- 4-bit pools
+
+namespace {
+
+bool fp4_head_dim(int dh) { return dh == 64 || dh == 128 || dh == 256; }
+
+// Shapes shared by the row operators; MLB_OK or a status.
+int row_shapes(const char* what, int dtype, int64_t num_tokens, int num_heads, int num_kv_heads, int head_dim) {
+  if (!elt_bytes(dtype)) return fail(MLB_EINVAL, "%s: unknown dtype %d", what, dtype);
+  if (num_tokens < 0 || num_heads < 0 || num_kv_heads < 0 || num_heads + num_kv_heads <= 0)
+    return fail(MLB_EINVAL, "%s: bad sizes", what);
+  if (!fp4_head_dim(head_dim)) return fail(MLB_EUNSUPPORTED, "%s: head_dim %d (supported: 64, 128, 256)", what, head_dim);
+  if (num_tokens > (int64_t(1) << 31) / std::max(1, num_heads + 2 * num_kv_heads))
+    return fail(MLB_EINVAL, "%s: %lld tokens of %d heads are too many rows for one launch", what,
+                static_cast<long long>(num_tokens), num_heads + 2 * num_kv_heads);
+  return MLB_OK;
+}
+
+int fp4_pools(const char* what, const void* k_cache, const void* v_cache, int64_t num_blocks, const void* slots,
+              int num_kv_heads) {
+  if (num_blocks <= 0 || num_kv_heads <= 0) return fail(MLB_EINVAL, "%s: bad pool sizes", what);
+  if (!k_cache || !v_cache || !slots) return fail(MLB_EINVAL, "%s: null pointer", what);
+  if (!aligned(k_cache, 16) || !aligned(v_cache, 16)) return fail(MLB_EINVAL, "%s: pools must be 16-byte aligned", what);
+  return MLB_OK;
+}
+
+bool rows_aligned(const void* p, int64_t st, int64_t sh, int eb) {
+  return aligned(p, 16) && (st * eb) % 16 == 0 && (sh * eb) % 16 == 0;
+}
+
+int rope_call(const char* what, mlb::RowArgs& a, int dtype, int head_dim, bool append, void* stream) {
+  const int eb = elt_bytes(dtype);
+  if (a.rot < 0 || a.rot > head_dim || a.rot % 16)
+    return fail(MLB_EUNSUPPORTED, "%s: rot_dim %d (a multiple of 16, at most head_dim %d)", what, a.rot, head_dim);
+  if (append && a.rot != head_dim)
+    return fail(MLB_EUNSUPPORTED, "%s: rot_dim %d: one launch needs the whole head rotated (%d)", what, a.rot, head_dim);
+  if (!(a.eps >= 0.f)) return fail(MLB_EINVAL, "%s: eps must not be negative", what);
+  if (a.num_positions < 0) return fail(MLB_EINVAL, "%s: bad sizes", what);
+  if (a.num_tokens == 0) return MLB_OK;
+  if ((a.h && (!a.q || !a.q_out)) || (a.hkv && (!a.k || (append ? !a.v : !a.k_out))) || !a.positions || (a.rot && !a.cos_sin))
+    return fail(MLB_EINVAL, "%s: null pointer", what);
+  if (!aligned(a.cos_sin, 16) || !aligned(a.q_weight, 16) || !aligned(a.k_weight, 16))
+    return fail(MLB_EINVAL, "%s: the table and the weights must be 16-byte aligned", what);
+  a.vec = (!a.h || (rows_aligned(a.q, a.q_st, a.q_sh, eb) && rows_aligned(a.q_out, a.qo_st, a.qo_sh, eb))) &&
+          (!a.hkv || (rows_aligned(a.k, a.k_st, a.k_sh, eb) &&
+                      (append ? rows_aligned(a.v, a.v_st, a.v_sh, eb) : rows_aligned(a.k_out, a.ko_st, a.ko_sh, eb))));
+  return cuda_status(mlb::launch_norm_rope(a, dtype, head_dim, append, sm_count(), static_cast<cudaStream_t>(stream)),
+                     what);
+}
+
+}  // namespace
+
+extern "C" {
+
+int mlb_qk_norm_rope(const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k, int64_t k_stride_tok,
+                     int64_t k_stride_head, int dtype, int64_t num_tokens, int num_heads, int num_kv_heads,
+                     int head_dim, const int64_t* positions, const float* cos_sin, int64_t num_positions, int rot_dim,
+                     const void* q_weight, const void* k_weight, float eps, void* q_out, int64_t q_out_stride_tok,
+                     int64_t q_out_stride_head, void* k_out, int64_t k_out_stride_tok, int64_t k_out_stride_head,
+                     int32_t* err_word, void* stream) {
+  if (int rc = row_shapes("qk_norm_rope", dtype, num_tokens, num_heads, num_kv_heads, head_dim)) return rc;
+  mlb::RowArgs a{};
+  a.q = static_cast<const char*>(q), a.q_st = q_stride_tok, a.q_sh = q_stride_head;
+  a.k = static_cast<const char*>(k), a.k_st = k_stride_tok, a.k_sh = k_stride_head;
+  a.q_out = static_cast<char*>(q_out), a.qo_st = q_out_stride_tok, a.qo_sh = q_out_stride_head;
+  a.k_out = static_cast<char*>(k_out), a.ko_st = k_out_stride_tok, a.ko_sh = k_out_stride_head;
+  a.num_tokens = num_tokens, a.h = num_heads, a.hkv = num_kv_heads, a.rot = rot_dim;
+  a.positions = positions, a.cos_sin = cos_sin, a.num_positions = num_positions;
+  a.q_weight = static_cast<const char*>(q_weight), a.k_weight = static_cast<const char*>(k_weight), a.eps = eps;
+  a.err = err_word;
+  return rope_call("qk_norm_rope", a, dtype, head_dim, false, stream);
+}
+
+int mlb_qk_norm_rope_append_fp4(const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k,
+                                int64_t k_stride_tok, int64_t k_stride_head, const void* v, int64_t v_stride_tok,
+                                int64_t v_stride_head, int dtype, int64_t num_tokens, int num_heads, int num_kv_heads,
+                                int head_dim, const int64_t* positions, const float* cos_sin, int64_t num_positions,
+                                int rot_dim, const void* q_weight, const void* k_weight, float eps, void* q_out,
+                                int64_t q_out_stride_tok, int64_t q_out_stride_head, void* k_cache, void* v_cache,
+                                int64_t num_blocks, const int64_t* slot_mapping, int32_t* err_word, void* stream) {
+  const char* what = "qk_norm_rope_append_fp4";
+  if (int rc = row_shapes(what, dtype, num_tokens, num_heads, num_kv_heads, head_dim)) return rc;
+  if (num_tokens)
+    if (int rc = fp4_pools(what, k_cache, v_cache, num_blocks, slot_mapping, num_kv_heads)) return rc;
+  mlb::RowArgs a{};
+  a.q = static_cast<const char*>(q), a.q_st = q_stride_tok, a.q_sh = q_stride_head;
+  a.k = static_cast<const char*>(k), a.k_st = k_stride_tok, a.k_sh = k_stride_head;
+  a.v = static_cast<const char*>(v), a.v_st = v_stride_tok, a.v_sh = v_stride_head;
+  a.q_out = static_cast<char*>(q_out), a.qo_st = q_out_stride_tok, a.qo_sh = q_out_stride_head;
+  a.num_tokens = num_tokens, a.h = num_heads, a.hkv = num_kv_heads, a.rot = rot_dim;
+  a.positions = positions, a.cos_sin = cos_sin, a.num_positions = num_positions;
+  a.q_weight = static_cast<const char*>(q_weight), a.k_weight = static_cast<const char*>(k_weight), a.eps = eps;
+  a.k_cache = static_cast<uint8_t*>(k_cache), a.v_cache = static_cast<uint8_t*>(v_cache);
+  a.slots = slot_mapping, a.num_slots = num_blocks * mlb::kBlockSize;
+  a.err = err_word;
+  return rope_call(what, a, dtype, head_dim, true, stream);
+}
+
+int mlb_kv_append_fp4(void* k_cache, void* v_cache, int64_t num_blocks, const int64_t* slot_mapping, const void* k,
+                      int64_t k_stride_tok, int64_t k_stride_head, const void* v, int64_t v_stride_tok,
+                      int64_t v_stride_head, int in_dtype, int64_t num_tokens, int num_kv_heads, int head_dim,
+                      int32_t* err_word, void* stream) {
+  if (int rc = row_shapes("kv_append_fp4", in_dtype, num_tokens, 0, num_kv_heads, head_dim)) return rc;
+  if (num_tokens == 0) return MLB_OK;
+  if (int rc = fp4_pools("kv_append_fp4", k_cache, v_cache, num_blocks, slot_mapping, num_kv_heads)) return rc;
+  if (!k || !v) return fail(MLB_EINVAL, "kv_append_fp4: null pointer");
+  const int eb = elt_bytes(in_dtype);
+  mlb::RowArgs a{};
+  a.k = static_cast<const char*>(k), a.k_st = k_stride_tok, a.k_sh = k_stride_head;
+  a.v = static_cast<const char*>(v), a.v_st = v_stride_tok, a.v_sh = v_stride_head;
+  a.num_tokens = num_tokens, a.hkv = num_kv_heads;
+  a.k_cache = static_cast<uint8_t*>(k_cache), a.v_cache = static_cast<uint8_t*>(v_cache);
+  a.slots = slot_mapping, a.num_slots = num_blocks * mlb::kBlockSize;
+  a.vec = rows_aligned(k, k_stride_tok, k_stride_head, eb) && rows_aligned(v, v_stride_tok, v_stride_head, eb);
+  a.err = err_word;
+  return cuda_status(mlb::launch_fp4_append(a, in_dtype, head_dim, sm_count(), static_cast<cudaStream_t>(stream)),
+                     "kv_append_fp4 launch");
+}
+
+int mlb_kv_read_fp4(const void* k_cache, const void* v_cache, int64_t num_blocks, const int64_t* slot_mapping,
+                    void* k_out, void* v_out, int out_dtype, int64_t num_tokens, int num_kv_heads, int head_dim,
+                    int32_t* err_word, void* stream) {
+  if (int rc = row_shapes("kv_read_fp4", out_dtype, num_tokens, 0, num_kv_heads, head_dim)) return rc;
+  if (num_tokens == 0) return MLB_OK;
+  if (int rc = fp4_pools("kv_read_fp4", k_cache, v_cache, num_blocks, slot_mapping, num_kv_heads)) return rc;
+  if (!k_out || !v_out) return fail(MLB_EINVAL, "kv_read_fp4: null pointer");
+  if (!aligned(k_out, 16) || !aligned(v_out, 16)) return fail(MLB_EINVAL, "kv_read_fp4: outputs must be 16-byte aligned");
+  mlb::RowArgs a{};
+  a.k_out = static_cast<char*>(k_out), a.q_out = static_cast<char*>(v_out);
+  a.num_tokens = num_tokens, a.hkv = num_kv_heads;
+  a.k_cache = static_cast<uint8_t*>(const_cast<void*>(k_cache));  // read only
+  a.v_cache = static_cast<uint8_t*>(const_cast<void*>(v_cache));
+  a.slots = slot_mapping, a.num_slots = num_blocks * mlb::kBlockSize;
+  a.err = err_word;
+  return cuda_status(mlb::launch_fp4_read(a, out_dtype, head_dim, sm_count(), static_cast<cudaStream_t>(stream)),
+                     "kv_read_fp4 launch");
+}
+
+int mlb_paged_attention_fp4(const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k_cache,
+                            const void* v_cache, int dtype, int64_t num_blocks, int num_heads, int num_kv_heads,
+                            int head_dim, float scale, const int32_t* block_tables, int64_t bt_stride,
+                            const int32_t* seq_lens, const int32_t* qo_indptr, int num_seqs,
+                            const mlb_work_unit* units, int64_t num_units, const mlb_shared_unit* shared_units,
+                            int64_t num_shared_units, const mlb_share_member* members, float* partial_o,
+                            float* partial_lse, int64_t num_partial_rows, void* out, int64_t out_stride_tok,
+                            int64_t out_stride_head, const mlb_out_targets* out_targets, int32_t* err_word,
+                            void* stream) {
+  const char* what = "paged_attention_fp4";
+  if (dtype != MLB_F16 && dtype != MLB_BF16)
+    return fail(MLB_EUNSUPPORTED, "%s: queries must be 16-bit (dtype %d)", what, dtype);
+  if (!fp4_head_dim(head_dim)) return fail(MLB_EUNSUPPORTED, "%s: head_dim %d (supported: 64, 128, 256)", what, head_dim);
+  if (num_kv_heads <= 0 || num_heads <= 0 || num_heads % num_kv_heads)
+    return fail(MLB_EINVAL, "%s: num_heads %d not a multiple of num_kv_heads %d", what, num_heads, num_kv_heads);
+  if (num_heads / num_kv_heads > 8)
+    return fail(MLB_EUNSUPPORTED, "%s: %d query heads per KV head (at most 8)", what, num_heads / num_kv_heads);
+  if (!(scale > 0.f) || !(scale <= 3.4028235e38f)) return fail(MLB_EINVAL, "%s: scale must be positive and finite", what);
+  if (num_units < 0 || num_shared_units < 0 || num_seqs < 0 || num_blocks <= 0 || num_partial_rows < 0)
+    return fail(MLB_EINVAL, "%s: bad sizes", what);
+  if (num_units == 0 && num_shared_units == 0) return MLB_OK;
+  if (!q || !k_cache || !v_cache || !block_tables || !seq_lens || !qo_indptr || (num_units && !units) ||
+      (num_shared_units && !shared_units))
+    return fail(MLB_EINVAL, "%s: null pointer", what);
+  if (num_shared_units % 2) return fail(MLB_EINVAL, "%s: query-tile units come in pairs", what);
+  mlb_out_targets targets;
+  if (int rc = resolve_targets(what, out, out_stride_tok, out_stride_head, out_targets, &targets)) return rc;
+  if (num_partial_rows > 0 && (!partial_o || !partial_lse))
+    return fail(MLB_EINVAL, "%s: the plan has %lld partial rows but no workspace", what,
+                static_cast<long long>(num_partial_rows));
+  if (!aligned(k_cache, 16) || !aligned(v_cache, 16)) return fail(MLB_EINVAL, "%s: pools must be 16-byte aligned", what);
+  if (num_units > INT32_MAX / num_kv_heads || num_shared_units > INT32_MAX / num_kv_heads)
+    return fail(MLB_EINVAL, "%s: grid too large", what);
+  mlb::AttnArgs a{};
+  a.q = static_cast<const char*>(q), a.q_st = q_stride_tok, a.q_sh = q_stride_head;
+  a.k_cache = static_cast<const char*>(k_cache), a.v_cache = static_cast<const char*>(v_cache);
+  a.num_blocks = num_blocks;
+  a.h = num_heads, a.hkv = num_kv_heads, a.group = num_heads / num_kv_heads;
+  a.tile_tokens = mlb::tokens_per_tile(num_heads, num_kv_heads);
+  a.sl2 = scale * mlb::kLog2e;
+  a.bt = block_tables, a.bt_stride = bt_stride, a.seq_lens = seq_lens, a.qo = qo_indptr;
+  a.units = units, a.shared_units = shared_units, a.members = members;
+  a.part_o = partial_o, a.part_lse = partial_lse, a.part_rows = num_partial_rows;
+  a.out = targets;
+  a.out_vec = mlb::out_vec_ok(targets, 2) ? 1 : 0;
+  a.q_vec = rows_aligned(q, q_stride_tok, q_stride_head, 2) ? 1 : 0;
+  a.err = err_word;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (num_shared_units > 0) {
+    const int rc = cuda_status(mlb::launch_fp4_shared(a, dtype, head_dim, num_shared_units, st), what);
+    if (rc != MLB_OK || num_units == 0) return rc;
+  }
+  return cuda_status(mlb::launch_fp4_attention(a, dtype, head_dim, num_units, st), what);
 }
 
 }  // extern "C"

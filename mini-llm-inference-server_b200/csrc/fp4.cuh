@@ -1,0 +1,91 @@
+// The 4-bit pool format and its conversions.
+//
+// A pool is uint8 [num_blocks][Hkv][17][Dh / 2]: one contiguous record per (block, head), so a page of one head
+// is a single run of 8.5 Dh bytes (1088 for Dh 128; 0.266 of the 16-bit page).  Rows 0..15 are the tokens' codes,
+// two e2m1 values a byte (dim 2i in the low nibble).  Row 16 holds the scales, one byte for each run of 32 dims
+// of a token, at [run][2 * (token % 8) + token / 8]: the byte of token g next to token g + 8's, the pair of rows
+// that one thread of a tensor-core fragment holds.  A scale byte b stands for the fp16 with bits b << 7 (5
+// exponent and 3 mantissa bits, no sign), so widening it is a shift.
+// value = code * scale: e2m1 has 2 significant bits and the scale 4, so a value has at most 6 and is exact in
+// bf16 and fp16 (6 * the largest scale, 61440, is a finite fp16; the smallest step, 2^-18, an fp16 subnormal).
+#pragma once
+
+#include "common.cuh"
+
+namespace mlb {
+
+constexpr int kFp4Run = 32;                // dims that share a scale
+constexpr float kFp4TopValue = 61440.f;    // 6 * the largest scale (10240): larger magnitudes are stored as this
+constexpr int kFp4Rows = kBlockSize + 1;   // 16 rows of codes, one of scales
+
+template <int DH>
+struct Fp4 {
+  static constexpr int kRow = DH / 2;                    // bytes of one token's codes
+  static constexpr int kScales = kBlockSize * kRow;      // offset of the scale row
+  static constexpr int kRecord = kFp4Rows * kRow;        // one (block, head)
+  static_assert(kRecord % 16 == 0, "records start 16-byte aligned");
+};
+
+// offset of a scale byte in the scale row
+__host__ __device__ constexpr int fp4_scale_at(int run, int token) { return run * kBlockSize + 2 * (token & 7) + (token >> 3); }
+
+// 8 codes (one 32-bit word) -> 4 pairs of fp16, dims in order
+__device__ __forceinline__ void fp4_unpack8(uint32_t w, uint32_t& h0, uint32_t& h1, uint32_t& h2, uint32_t& h3) {
+  asm("{\n.reg .b8 b0, b1, b2, b3;\nmov.b32 {b0, b1, b2, b3}, %4;\n"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\ncvt.rn.f16x2.e2m1x2 %1, b1;\n"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\ncvt.rn.f16x2.e2m1x2 %3, b3;\n}\n"
+      : "=r"(h0), "=r"(h1), "=r"(h2), "=r"(h3)
+      : "r"(w));
+}
+
+__device__ __forceinline__ uint32_t hmul2_u32(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+
+// 8 values -> one word of codes; nearest level, ties to even codes (cvt), sign kept
+__device__ __forceinline__ uint32_t fp4_pack8(const float (&r)[8]) {
+  uint32_t w;
+  asm("{\n.reg .b8 b0, b1, b2, b3;\n"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\ncvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n"
+      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\ncvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n"
+      "mov.b32 %0, {b0, b1, b2, b3};\n}\n"
+      : "=r"(w)
+      : "f"(r[0]), "f"(r[1]), "f"(r[2]), "f"(r[3]), "f"(r[4]), "f"(r[5]), "f"(r[6]), "f"(r[7]));
+  return w;
+}
+
+// Scale byte of a run whose largest finite magnitude is amax (clamped to kFp4TopValue by the caller):
+// amax / 6 rounded once to the byte format, ties to even.  The quotient is cut (towards zero) and its last bit set
+// when anything was cut off, so the second rounding sees which side of a tie the true quotient lies on.
+__device__ __forceinline__ uint32_t fp4_scale_byte(float amax) {
+  float y = __fdiv_rz(amax, 6.f);
+  if (fmaf(-y, 6.f, amax) != 0.f) y = __uint_as_float(__float_as_uint(y) | 1u);
+  if (y < 6.103515625e-05f) return static_cast<uint32_t>(rintf(y * 131072.f));  // below 2^-14: steps of 2^-17
+  uint32_t u = __float_as_uint(y);
+  u += 0x7ffffu + ((u >> 20) & 1u);       // to 3 mantissa bits, nearest even
+  return (u >> 20) - ((127u - 15u) << 3);  // exponent bias 15
+}
+
+__device__ __forceinline__ float fp4_scale_value(uint32_t byte) {
+  return __half2float(__ushort_as_half(static_cast<unsigned short>(byte << 7)));
+}
+
+// x / scale with rounding that never moves a value onto a border between two levels: the Newton step makes exact
+// quotients exact (a border times a scale has 7 significant bits); for fp32 inputs, whose quotients can round onto
+// a border they only lie next to, an inexact quotient is made odd in the direction of its remainder.
+template <bool WIDE>
+__device__ __forceinline__ float fp4_quotient(float x, float scale, float inv) {
+  float q = x * inv;
+  q = fmaf(fmaf(-q, scale, x), inv, q);
+  if constexpr (WIDE) {
+    const float r = fmaf(-q, scale, x);
+    uint32_t u = __float_as_uint(q);
+    if (r != 0.f && !(u & 1u) && (u << 1) != 0u) u += ((__float_as_uint(r) ^ u) >> 31) ? 0xffffffffu : 1u;
+    q = __uint_as_float(u);
+  }
+  return copysignf(q, x);  // the correction would turn -0 into +0
+}
+
+}  // namespace mlb

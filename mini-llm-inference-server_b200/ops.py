@@ -8,6 +8,7 @@ error word instead of faulting the GPU.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 from dataclasses import dataclass
@@ -123,13 +124,15 @@ def _i32(a) -> np.ndarray:
 
 def plan_attention(qo_indptr: list[int], seq_lens: list[int], max_blocks: int, num_heads: int, num_kv_heads: int,
                    device: torch.device | str, block_size: int = BLOCK_SIZE, num_sms: int | None = None,
-                   pages_per_unit: int = 0, block_tables_host: np.ndarray | None = None) -> AttentionPlan:
+                   pages_per_unit: int = 0, block_tables_host: np.ndarray | None = None,
+                   pool_dtype: torch.dtype | None = None) -> AttentionPlan:
     """Split the step into units (host work, like FlashInfer's plan(); flashinfer_backend.py:48-64).
 
     qo_indptr / seq_lens are the host lists AttentionMetadata keeps (metadata.py:39-40), so planning
     needs no device round trip.  With `block_tables_host` (int32 [S, W]) decode rows that share leading
-    blocks (prefix-cache hits) are planned as shared-prefix units (16-bit pools only).  The plan is copied
-    to the device in one transfer.
+    blocks (prefix-cache hits) are planned as shared-prefix units (16-bit and 4-bit pools only).  The plan is
+    copied to the device in one transfer.  `pool_dtype` torch.uint8: the plan is for 4-bit pools
+    (`paged_attention_fp4`); any plan is right for any pool, the split size is what differs.
     """
     device = torch.device(device)
     qo, lens = _i32(qo_indptr), _i32(seq_lens)
@@ -358,6 +361,281 @@ def _strides(out: torch.Tensor | None) -> tuple[int, int]:
 
 def _targets(t: OutTargets | None):
     return ctypes.byref(t) if t is not None else None
+
+
+# ---------------------------------------------------------------- 4-bit pools
+
+FP4_ROWS = BLOCK_SIZE + 1  # rows of a (block, head): 16 tokens' codes, then their scales
+FP4_RUN = 32  # dims that share a scale
+
+
+def is_fp4(pool: torch.Tensor) -> bool:
+    """Whether `pool` is a 4-bit pool (uint8 [num_blocks, Hkv, 17, Dh / 2], see include/mlb_paged_kv.h)."""
+    return pool.dtype is torch.uint8
+
+
+def pool_kv_heads(pool: torch.Tensor) -> int:
+    return pool.shape[1] if is_fp4(pool) else pool.shape[2]
+
+
+def fp4_pool_shape(num_blocks: int, num_kv_heads: int, head_dim: int) -> tuple[int, int, int, int]:
+    """Shape of a 4-bit pool: 8.5 x head_dim bytes per (block, head) instead of 32 x head_dim in 16 bits."""
+    if head_dim not in (64, 128, 256):
+        raise ValueError(f"4-bit pools: head_dim {head_dim} (supported: 64, 128, 256)")
+    return num_blocks, num_kv_heads, FP4_ROWS, head_dim // 2
+
+
+def _on(device: torch.device):
+    """The launches' device made current, if it is not already."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _check_fp4_pools(k_cache: torch.Tensor, v_cache: torch.Tensor, what: str) -> tuple[int, int, int]:
+    """(num_blocks, Hkv, Dh) of a pair of 4-bit pools."""
+    _check_pool(k_cache, what)
+    _check_pool(v_cache, what)
+    if k_cache.dtype is not torch.uint8 or k_cache.shape[2] != FP4_ROWS:
+        raise ValueError(f"{what}: 4-bit pools are uint8 [num_blocks, Hkv, {FP4_ROWS}, Dh / 2], got {k_cache.dtype} "
+                         f"{tuple(k_cache.shape)}")
+    if v_cache.shape != k_cache.shape or v_cache.dtype is not torch.uint8 or v_cache.device != k_cache.device:
+        raise ValueError(f"{what}: k_cache and v_cache differ")
+    return k_cache.shape[0], k_cache.shape[1], 2 * k_cache.shape[3]
+
+
+def _check_index(t: torch.Tensor, n: int, device: torch.device, what: str) -> None:
+    if t.dtype is not torch.long or t.shape != (n,) or not t.is_contiguous() or t.device != device:
+        raise ValueError(f"{what} must be a contiguous int64 [{n}] tensor on {device}, got {t.dtype} {tuple(t.shape)} "
+                         f"on {t.device}")
+
+
+def kv_append_fp4(k_cache: torch.Tensor, v_cache: torch.Tensor, slot_mapping: torch.Tensor, k: torch.Tensor,
+                  v: torch.Tensor, err: torch.Tensor | None = None) -> None:
+    """`kv_append` into 4-bit pools: rows k[i] / v[i] (float32, float16 or bfloat16, strided views allowed) are
+    rounded to e2m1 codes with a scale for each 32 dims (mlb_kv_append_fp4) and stored at slot_mapping[i].  Slots
+    must be distinct."""
+    nb, hkv, dh = _check_fp4_pools(k_cache, v_cache, "kv_append_fp4")
+    _check_rows(k, hkv, dh, "kv_append_fp4 k")
+    _check_rows(v, hkv, dh, "kv_append_fp4 v")
+    n = k.shape[0]
+    if v.shape[0] != n or k.dtype != v.dtype:
+        raise ValueError(f"kv_append_fp4: k and v differ ({tuple(k.shape)} {k.dtype}, {tuple(v.shape)} {v.dtype})")
+    if k.device != k_cache.device or v.device != k_cache.device:
+        raise ValueError("kv_append_fp4: all tensors must be on the pools' device")
+    _check_index(slot_mapping, n, k_cache.device, "kv_append_fp4: slot_mapping")
+    code = _code(k, "kv_append_fp4")
+    if n == 0:
+        return
+    with _on(k_cache.device):
+        rc = lib().mlb_kv_append_fp4(k_cache.data_ptr(), v_cache.data_ptr(), nb, slot_mapping.data_ptr(), k.data_ptr(),
+                                     k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), code, n, hkv,
+                                     dh, _ptr(err), _stream(k_cache.device))
+    check(rc, "kv_append_fp4")
+
+
+def kv_read_fp4(k_cache: torch.Tensor, v_cache: torch.Tensor, slot_mapping: torch.Tensor,
+                dtype: torch.dtype = torch.bfloat16, err: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The values that 4-bit pools hold at slot_mapping: (k, v) rows [N, Hkv, Dh] of `dtype` (exact in all three).
+    The same slot may be asked for more than once; a slot out of range reads as zeros."""
+    nb, hkv, dh = _check_fp4_pools(k_cache, v_cache, "kv_read_fp4")
+    if dtype not in DTYPE_CODE:
+        raise ValueError(f"kv_read_fp4: dtype {dtype} not supported (float32, float16, bfloat16)")
+    if slot_mapping.dim() != 1:
+        raise ValueError("kv_read_fp4: slot_mapping must be 1-D")
+    n = slot_mapping.shape[0]
+    _check_index(slot_mapping, n, k_cache.device, "kv_read_fp4: slot_mapping")
+    k = torch.empty((n, hkv, dh), dtype=dtype, device=k_cache.device)
+    v = torch.empty_like(k)
+    if n:
+        with _on(k_cache.device):
+            rc = lib().mlb_kv_read_fp4(k_cache.data_ptr(), v_cache.data_ptr(), nb, slot_mapping.data_ptr(),
+                                       k.data_ptr(), v.data_ptr(), DTYPE_CODE[dtype], n, hkv, dh, _ptr(err),
+                                       _stream(k_cache.device))
+        check(rc, "kv_read_fp4")
+    return k, v
+
+
+def attention_partials_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+                           seq_lens: torch.Tensor, qo_indptr: torch.Tensor, plan: AttentionPlan,
+                           workspace: Workspace, out: torch.Tensor | None = None, scale: float | None = None,
+                           err: torch.Tensor | None = None, targets: OutTargets | None = None) -> torch.Tensor | None:
+    """`attention_partials` over 4-bit pools: unsplit rows are final in `out` (or `targets`), split ones leave
+    partial rows in `workspace` for `splitk_reduce`."""
+    what = "paged_attention_fp4"
+    nb, hkv, dh = _check_fp4_pools(k_cache, v_cache, what)
+    if q.dim() != 3 or q.shape[2] != dh or (q.shape[0] and q.stride(2) != 1):
+        raise ValueError(f"{what}: q must be [N, H, {dh}] with unit last stride, got {tuple(q.shape)}")
+    if q.dtype is not torch.bfloat16 and q.dtype is not torch.float16:
+        raise ValueError(f"{what}: q must be float16 or bfloat16, got {q.dtype}")
+    n, h = q.shape[0], q.shape[1]
+    if (plan.num_heads, plan.num_kv_heads, plan.num_tokens) != (h, hkv, n):
+        raise ValueError(f"{what}: the plan was built for another shape")
+    if q.device != k_cache.device:
+        raise ValueError(f"{what}: q must be on the pools' device")
+    for t, name in ((block_tables, "block_tables"), (seq_lens, "seq_lens"), (qo_indptr, "qo_indptr"),
+                    (plan.units, "the plan")):
+        if t.dtype is not torch.int32 or not t.is_contiguous() or t.device != q.device:
+            raise ValueError(f"{what}: {name} must be a contiguous int32 tensor on {q.device}")
+    if targets is not None:
+        out = None
+    elif out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or (n and out.stride(2) != 1):
+        raise ValueError(f"{what}: out must match q")
+    if n == 0 or plan.num_units + plan.num_shared_units == 0:
+        return out
+    scale = 1.0 / math.sqrt(dh) if scale is None else float(scale)
+    po = plse = None
+    if plan.num_partial_rows:
+        po, plse = workspace.get(plan.num_partial_rows, h, dh, q.device)
+    with _on(q.device):
+        rc = lib().mlb_paged_attention_fp4(
+            q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), DTYPE_CODE[q.dtype], nb, h,
+            hkv, dh, scale, block_tables.data_ptr(), block_tables.stride(0), seq_lens.data_ptr(), qo_indptr.data_ptr(),
+            seq_lens.shape[0], plan.units.data_ptr(), plan.num_units, plan.shared_units.data_ptr(),
+            plan.num_shared_units, plan.members.data_ptr(), _ptr(po), _ptr(plse), plan.num_partial_rows, _ptr(out),
+            *_strides(out), _targets(targets), _ptr(err), _stream(q.device))
+    check(rc, what)
+    return out
+
+
+def paged_attention_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+                        seq_lens: torch.Tensor, qo_indptr: torch.Tensor, plan: AttentionPlan,
+                        workspace: Workspace | None = None, out: torch.Tensor | None = None,
+                        scale: float | None = None, err: torch.Tensor | None = None,
+                        targets: OutTargets | None = None) -> torch.Tensor | None:
+    """`paged_attention` over 4-bit pools: q [N, H, Dh] float16 or bfloat16 -> [N, H, Dh] in q's dtype, the pools
+    holding this step's rows already (`kv_append_fp4`).  Same metadata tensors, plan and workspace."""
+    workspace = workspace or Workspace()
+    out = attention_partials_fp4(q, k_cache, v_cache, block_tables, seq_lens, qo_indptr, plan, workspace, out, scale,
+                                 err, targets)
+    with _on(q.device):
+        splitk_reduce(plan, workspace, out, targets, q.dtype, q.shape[2], q.device)
+    return out
+
+
+# ---------------------------------------------------------------- norm and rotation of queries and keys
+
+
+def rotary_table(num_positions: int, rot_dim: int, theta: float = 500000.0, device: torch.device | str = "cuda",
+                 inv_freq: torch.Tensor | None = None) -> torch.Tensor:
+    """The rotation table of `qk_norm_rope`: float32 [num_positions, rot_dim], cos of each position's rot_dim / 2
+    angles, then their sin.  Angles are formed in 64 bits (position x frequency needs more than 32 at far
+    positions).  `inv_freq` [rot_dim / 2] replaces theta^(-2i / rot_dim) (a model's scaled frequencies)."""
+    if rot_dim <= 0 or rot_dim % 16 or num_positions <= 0:
+        raise ValueError(f"rotary_table: rot_dim {rot_dim} must be a positive multiple of 16, num_positions "
+                         f"{num_positions} positive")
+    if inv_freq is None:
+        inv_freq = theta ** (-torch.arange(0, rot_dim, 2, dtype=torch.float64) / rot_dim)
+    elif inv_freq.shape != (rot_dim // 2,):
+        raise ValueError(f"rotary_table: inv_freq must be [{rot_dim // 2}], got {tuple(inv_freq.shape)}")
+    inv = inv_freq.to(device=device, dtype=torch.float64)
+    angle = torch.arange(num_positions, dtype=torch.float64, device=device)[:, None] * inv
+    return torch.cat([angle.cos(), angle.sin()], dim=1).float()
+
+
+@dataclass
+class Rotary:
+    """What a layer does to its queries and keys before attention: the table, and the weights of the norms of the
+    query and key heads (None: no norm)."""
+
+    cos_sin: torch.Tensor
+    q_weight: torch.Tensor | None = None
+    k_weight: torch.Tensor | None = None
+    eps: float = 1e-6
+
+
+def _check_rope(what: str, q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor,
+                q_weight: torch.Tensor | None, k_weight: torch.Tensor | None) -> int:
+    if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
+        raise ValueError(f"{what}: q must be [N, H, Dh] and k [N, Hkv, Dh], got {tuple(q.shape)}, {tuple(k.shape)}")
+    dh = q.shape[2]
+    _check_rows(q, q.shape[1], dh, what)
+    _check_rows(k, k.shape[1], dh, what)
+    if q.dtype != k.dtype or q.device != k.device or not q.is_cuda:
+        raise ValueError(f"{what}: q and k must be CUDA tensors of one dtype on one device")
+    if dh not in (64, 128, 256):
+        raise ValueError(f"{what}: head_dim {dh} (supported: 64, 128, 256)")
+    _check_index(positions, q.shape[0], q.device, f"{what}: positions")
+    if (cos_sin.dtype is not torch.float32 or cos_sin.dim() != 2 or not cos_sin.is_contiguous()
+            or cos_sin.device != q.device):
+        raise ValueError(f"{what}: cos_sin must be a contiguous float32 [num_positions, rot_dim] tensor on {q.device}")
+    for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        if w is not None and (w.shape != (dh,) or w.dtype != q.dtype or w.device != q.device or not w.is_contiguous()):
+            raise ValueError(f"{what}: {name} must be a contiguous [{dh}] tensor of q's dtype on {q.device}")
+    return _code(q, what)
+
+
+def _check_row_out(what: str, out: torch.Tensor, x: torch.Tensor) -> None:
+    if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
+        raise ValueError(f"{what}: out must match its input, got {tuple(out.shape)} {out.dtype} on {out.device}")
+    if out.numel() == 0:
+        return
+    n, h, dh = out.shape
+    a, b = sorted([(out.stride(0), n), (out.stride(1), h)])
+    if out.stride(2) != 1 or (a[1] > 1 and a[0] < dh) or (b[1] > 1 and b[0] < max(a[0] * (a[1] - 1), 0) + dh):
+        raise ValueError(f"{what}: out rows must not overlap, got strides {out.stride()}")
+    if out.data_ptr() == x.data_ptr() and out.stride() != x.stride():
+        raise ValueError(f"{what}: out on the memory of its input must have its strides")
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor,
+                 q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 1e-6,
+                 out: tuple[torch.Tensor, torch.Tensor] | None = None,
+                 err: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Norm of each query and key head (weights [Dh] of q's dtype; None: no norm) and their rotation by position,
+    one launch (mlb_qk_norm_rope): q [N, H, Dh], k [N, Hkv, Dh] -> the same shapes and dtype, computed in fp32.
+    q and k may be views of a fused projection.  positions int64 [N] (AttentionMetadata.positions); cos_sin from
+    `rotary_table`, its rot_dim at most Dh (the dims behind it are not rotated).  out = (q_out, k_out) may be
+    (q, k)."""
+    what = "qk_norm_rope"
+    code = _check_rope(what, q, k, positions, cos_sin, q_weight, k_weight)
+    if out is None:
+        qo, ko = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k))
+    else:
+        qo, ko = out
+        _check_row_out(what, qo, q)
+        _check_row_out(what, ko, k)
+    n, h, dh = q.shape
+    with _on(q.device):
+        rc = lib().mlb_qk_norm_rope(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
+                                    code, n, h, k.shape[1], dh, positions.data_ptr(), cos_sin.data_ptr(),
+                                    cos_sin.shape[0], cos_sin.shape[1], _ptr(q_weight), _ptr(k_weight), eps,
+                                    qo.data_ptr(), qo.stride(0), qo.stride(1), ko.data_ptr(), ko.stride(0),
+                                    ko.stride(1), _ptr(err), _stream(q.device))
+    check(rc, what)
+    return qo, ko
+
+
+def qk_norm_rope_append_fp4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
+                            cos_sin: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                            slot_mapping: torch.Tensor, q_weight: torch.Tensor | None = None,
+                            k_weight: torch.Tensor | None = None, eps: float = 1e-6,
+                            out: torch.Tensor | None = None, err: torch.Tensor | None = None) -> torch.Tensor:
+    """`qk_norm_rope` and `kv_append_fp4` of its keys and of v in one launch: the cache and the returned queries are
+    bit-identical to the two calls'.  cos_sin must rotate the whole head (rot_dim == Dh)."""
+    what = "qk_norm_rope_append_fp4"
+    nb, hkv, dh = _check_fp4_pools(k_cache, v_cache, what)
+    code = _check_rope(what, q, k, positions, cos_sin, q_weight, k_weight)
+    n, h = q.shape[:2]
+    _check_rows(k, hkv, dh, f"{what} k")
+    _check_rows(v, hkv, dh, f"{what} v")
+    if v.shape[0] != n or v.dtype != k.dtype or v.device != k.device or k_cache.device != k.device:
+        raise ValueError(f"{what}: q, k, v and the pools must agree in rows, dtype and device")
+    _check_index(slot_mapping, n, q.device, f"{what}: slot_mapping")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    else:
+        _check_row_out(what, out, q)
+    with _on(q.device):
+        rc = lib().mlb_qk_norm_rope_append_fp4(
+            q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
+            v.stride(1), code, n, h, hkv, dh, positions.data_ptr(), cos_sin.data_ptr(), cos_sin.shape[0],
+            cos_sin.shape[1], _ptr(q_weight), _ptr(k_weight), eps, out.data_ptr(), out.stride(0), out.stride(1),
+            k_cache.data_ptr(), v_cache.data_ptr(), nb, slot_mapping.data_ptr(), _ptr(err), _stream(q.device))
+    check(rc, what)
+    return out
 
 
 # ---------------------------------------------------------------- metadata expansion on the device

@@ -26,7 +26,7 @@ import torch.distributed as dist
 
 from . import _lib
 from .attention.base import AttentionBackend
-from .ops import _stream, out_targets
+from .ops import _stream, out_targets, pool_kv_heads
 
 
 def head_range(rank: int, world: int, num_heads: int) -> slice:
@@ -246,8 +246,9 @@ class KVHeadShardedBackend(AttentionBackend):
     def forward(self, q, k, v, k_cache, v_cache, meta):
         qs = head_range(self.rank, self.world, q.shape[1])
         ks = head_range(self.rank, self.world, k.shape[1])
-        if k_cache.shape[2] != ks.stop - ks.start:
-            raise ValueError(f"rank {self.rank}: pools hold {k_cache.shape[2]} KV heads, expected {ks.stop - ks.start}")
+        if pool_kv_heads(k_cache) != ks.stop - ks.start:
+            raise ValueError(f"rank {self.rank}: pools hold {pool_kv_heads(k_cache)} KV heads, expected "
+                             f"{ks.stop - ks.start}")
         if self.transport == "p2p" and self.world > 1:
             return self._forward_p2p(q, k, v, k_cache, v_cache, meta, qs, ks)
         local = self.inner.forward(q[:, qs], k[:, ks], v[:, ks], k_cache, v_cache, meta)  # [N, H/n, Dh]
@@ -261,8 +262,8 @@ class KVHeadShardedBackend(AttentionBackend):
         h = q_l.shape[1] * self.world
         qs = head_range(self.rank, self.world, h)
         ks = head_range(self.rank, self.world, k_l.shape[1] * self.world)
-        if k_cache.shape[2] != k_l.shape[1]:
-            raise ValueError(f"rank {self.rank}: pools hold {k_cache.shape[2]} KV heads, k_l {k_l.shape[1]}")
+        if pool_kv_heads(k_cache) != k_l.shape[1]:
+            raise ValueError(f"rank {self.rank}: pools hold {pool_kv_heads(k_cache)} KV heads, k_l {k_l.shape[1]}")
         if self.transport == "p2p" and self.world > 1:
             return self._forward_p2p(q_l, k_l, v_l, k_cache, v_cache, meta, qs, ks, local=True)
         local = self.inner.forward(q_l, k_l, v_l, k_cache, v_cache, meta)
