@@ -153,12 +153,13 @@ typedef struct {
  * bt_stride_host; pass it for 16-bit pools only.  When given, decode rows whose tables start with the same
  * run of block ids (shared prefix blocks) get shared-prefix units (a cascade split), and rows of >= 16 new
  * tokens get query-tile units (kind 1 above) instead of 8-column work units.  pages_per_unit = 0 picks a
- * split size from the total work and num_sms.
+ * split size from the total work and num_sms for 16- and 32-bit pools, MLB_PAGES_PER_UNIT_FP4 one for 4-bit pools.
  * With units == NULL only the counts are returned (*num_units, *num_shared_units, *num_members,
  * *num_partial_rows); otherwise every output array must hold its count (MLB_ENOSPACE if not).
  * reduce_rows / reduce_chunks [num_tokens]: first partial row and number of pieces per token (pieces
  * <= 1: nothing to reduce).  Query tokens per tile = max(1, 8 / (num_heads / num_kv_heads)).
  */
+enum { MLB_PAGES_PER_UNIT_FP4 = -4 };
 MLB_API int mlb_plan_attention(const int32_t* qo_indptr, const int32_t* seq_lens, int num_seqs, int max_blocks_per_seq,
                        const int32_t* block_tables_host, int64_t bt_stride_host,
                        int num_heads, int num_kv_heads, int block_size, int num_sms, int pages_per_unit,
@@ -461,6 +462,16 @@ MLB_API int mlb_paged_attention_fp4(const void* q, int64_t q_stride_tok, int64_t
                       const mlb_share_member* members, float* partial_o, float* partial_lse,
                       int64_t num_partial_rows, void* out, int64_t out_stride_tok, int64_t out_stride_head,
                       const mlb_out_targets* out_targets, int32_t* err_word, void* stream);
+
+/*
+ * mlb_splitk_reduce for few tokens of many pieces: one CTA per (token, head) shares the pieces between its warps.
+ * Same arguments and contract; the sums are taken in another order.  A NaN partial row gives a NaN row.
+ */
+MLB_API int mlb_splitk_reduce_wide(const float* partial_o, const float* partial_lse, int64_t num_partial_rows,
+                      const int32_t* reduce_rows, const int32_t* reduce_chunks, int tokens_per_tile,
+                      int64_t num_tokens, int num_heads, int head_dim,
+                      void* out, int64_t out_stride_tok, int64_t out_stride_head, int out_dtype,
+                      const mlb_out_targets* out_targets, void* stream);
 
 #ifdef __cplusplus
 }

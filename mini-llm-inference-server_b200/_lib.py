@@ -23,10 +23,12 @@ EXPORTS = ("mlb_last_error", "mlb_abi_version", "mlb_kv_append", "mlb_plan_atten
            "mlb_ipc_close", "mlb_ipc_free", "mlb_peer_barrier", "mlb_set_programmatic_launch",
            "mlb_splitk_reduce_gather", "mlb_set_tensor_core_prefix", "mlb_paged_attention_append",
            "mlb_build_metadata", "mlb_set_concurrent_prefix", "mlb_splitk_reduce_exchange", "mlb_kv_append_fp4",
-           "mlb_kv_read_fp4", "mlb_qk_norm_rope", "mlb_qk_norm_rope_append_fp4", "mlb_paged_attention_fp4")
+           "mlb_kv_read_fp4", "mlb_qk_norm_rope", "mlb_qk_norm_rope_append_fp4", "mlb_paged_attention_fp4",
+           "mlb_splitk_reduce_wide")
 ABI_VERSION = 10
 NOALLOC_SCRATCH_BYTES = 8 << 20  # MLB_NOALLOC_SCRATCH_BYTES
 MAX_OUT_DESTS = 8  # MLB_MAX_OUT_DESTS
+PAGES_PER_UNIT_FP4 = -4  # MLB_PAGES_PER_UNIT_FP4
 IPC_HANDLE_BYTES = 64  # MLB_IPC_HANDLE_BYTES
 
 
@@ -93,6 +95,8 @@ _SIGNATURES = {
                                            POINTER(AppendRows), c_void_p, c_void_p]),
     "mlb_splitk_reduce": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_int64, c_int, c_int,
                                   c_void_p, c_int64, c_int64, c_int, POINTER(OutTargets), c_void_p]),
+    "mlb_splitk_reduce_wide": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_int64, c_int, c_int,
+                                       c_void_p, c_int64, c_int64, c_int, POINTER(OutTargets), c_void_p]),
     "mlb_block_copy": (c_int, [c_void_p, c_int, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_void_p,
                                c_void_p]),
     "mlb_build_metadata": (c_int, [c_void_p, c_int64, c_int, c_int64, c_int64, c_int, c_int, c_void_p, c_void_p,

@@ -4,6 +4,7 @@
 #include <algorithm>
 #include <array>
 #include <atomic>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <string>
@@ -26,6 +27,9 @@ bool concurrent_prefix();  // mlb_set_concurrent_prefix
 cudaError_t launch_splitk_reduce(const float* po, const float* plse, const int32_t* rrows, const int32_t* rchunks,
                                  int tpt, int64_t ntok, int h, int dh, const mlb_out_targets& out,
                                  int out_dtype, cudaStream_t s);
+cudaError_t launch_splitk_reduce_wide(const float* po, const float* plse, const int32_t* rrows, const int32_t* rchunks,
+                                      int tpt, int64_t ntok, int h, int dh, const mlb_out_targets& out, int out_dtype,
+                                      cudaStream_t s);
 cudaError_t launch_splitk_reduce_gather(const float* po, const float* plse, const int32_t* rrows,
                                         const int32_t* rchunks, int tpt, int64_t ntok, int h, int dh,
                                         const mlb_out_targets& out, int self, int out_dtype, cudaStream_t s);
@@ -90,6 +94,60 @@ constexpr int kMinSharePages = 8;    // ... sharing at least this many full page
 constexpr int kPrefillMinTokens = 16;   // multi-token rows this long go to tensor-core query tiles ...
 constexpr int kPrefillPiecePages = 128;  // ... split into pieces of at most this many pages (16 MMA tiles)
 
+struct Group {
+  int seq, tile, pages;
+  int start = 0;  // pages before this are planned as shared-prefix units (0: none)
+  int shared_pieces = 0;
+};
+
+// Split size for the 4-bit kernel (pages_per_unit MLB_PAGES_PER_UNIT_FP4): the candidate with the shortest
+// estimated step.  A CTA's time is its pages plus a start and an end worth kFp4CtaPages pages; up to 4 CTAs are
+// resident per SM, and one with fewer neighbours runs faster (measured on B200, rows of 8 KV heads: 64 CTAs of 256
+// pages 28.7 us, 128 of 128 18.3, 256 of 64 16.4, 512 of 128 38.4); a split costs the reduction's launch and its
+// rows.  Units of one length: what counts is the SM with the most of them (16 x 131072 tokens: 768 CTAs 444 us,
+// 1152 405, 4096 395).  Of several lengths: 1 to 1.6 waves leave SMs idle at the end (64 rows of 512..4096 tokens:
+// 688 CTAs 43.5 us, 776 45.9, 1032 40.9, 1136 39.3; 4 KV heads: 568 24.9, 684 30.5).
+constexpr int kFp4CtasPerSm = 4;
+constexpr double kFp4CtaPages = 24, kFp4ReducePages = 13;
+constexpr double kFp4Alone[kFp4CtasPerSm + 1] = {2.15, 2.15, 1.4, 1.12, 1.0};  // speed by resident CTAs per SM
+
+int64_t fp4_pages_per_unit(const std::vector<Group>& groups, int hkv, int num_heads, int num_sms) {
+  const double slots = static_cast<double>(num_sms) * kFp4CtasPerSm;
+  int64_t longest = 0;
+  for (const Group& g : groups) longest = std::max<int64_t>(longest, g.pages - g.start);
+  int64_t best = std::max<int64_t>(longest, 1);
+  double best_time = -1;
+  for (int64_t c = 16; ; c += c < 64 ? 8 : c < 128 ? 16 : c < 256 ? 32 : c < 1024 ? 128 : 1024) {
+    const bool whole = c >= longest;
+    double sum = 0, top = 0, low = 1e30, rows = 0;
+    int64_t units = 0;
+    for (const Group& g : groups) {
+      const int64_t own = g.pages - g.start;
+      if (own <= 0) continue;
+      const int64_t k = (own + c - 1) / c;
+      const double t = static_cast<double>((own + k - 1) / k) + kFp4CtaPages;
+      units += k * hkv;
+      sum += t * static_cast<double>(k * hkv);
+      top = std::max(top, t);
+      low = std::min(low, t);
+      if (k > 1) rows += static_cast<double>(k);
+    }
+    double time;
+    if (units <= num_sms * kFp4CtasPerSm) {
+      time = top / kFp4Alone[(units + num_sms - 1) / num_sms];
+    } else if (top - low < 0.02 * top) {  // equal units: the SM with the most of them, and its last ones alone
+      time = static_cast<double>((units + num_sms - 1) / num_sms) * top / kFp4CtasPerSm + 0.12 * top;
+    } else {  // largest first: the smallest close the gaps, where there are enough of them
+      time = sum / slots * (static_cast<double>(units) < 1.6 * slots ? 1.18 : 1.0) + 0.5 * low;
+      time = std::max(time, top);
+    }
+    if (rows > 0) time += kFp4ReducePages + 8.8e-4 * rows * num_heads;
+    if (best_time < 0 || time < best_time) best_time = time, best = c;
+    if (whole || c > (int64_t(1) << 20)) break;
+  }
+  return best;
+}
+
 // The destinations of a call's final rows: its own `out`, or the caller's targets (checked).
 int resolve_targets(const char* what, void* out, int64_t st, int64_t sh, const mlb_out_targets* t,
                     mlb_out_targets* r) {
@@ -143,12 +201,6 @@ cudaError_t side_stream(SideStream** out) {
   *out = &s;
   return cudaSuccess;
 }
-
-struct Group {
-  int seq, tile, pages;
-  int start = 0;  // pages before this are planned as shared-prefix units (0: none)
-  int shared_pieces = 0;
-};
 
 // Sets of decode rows whose block tables begin with the same run of block ids (shared prefix-cache blocks).
 struct ShareSet {
@@ -377,7 +429,9 @@ int mlb_plan_attention(const int32_t* qo_indptr, const int32_t* seq_lens, int nu
   // - rows of one length (config 5, 29 x 8192 pages): a last wave under half full costs a whole unit time
   //   (4 heads: 1.31 waves 1358 us, 1.05 waves 1444, 1.57 waves 1190 = 1/2 of the 8-head time), so every row
   //   gets the same number of units and they fill ~1.55 waves.
-  int64_t chunk = pages_per_unit;
+  int64_t chunk = pages_per_unit == MLB_PAGES_PER_UNIT_FP4
+                      ? fp4_pages_per_unit(groups, num_kv_heads, num_heads, num_sms)
+                      : pages_per_unit;
   if (chunk <= 0) {
     const int64_t slots = static_cast<int64_t>(num_sms) * kCtasPerSm;
     const int64_t work = rest * num_kv_heads;  // page-heads left to the per-sequence kernel
@@ -968,6 +1022,9 @@ int mlb_paged_attention_fp4(const void* q, int64_t q_stride_tok, int64_t q_strid
     return fail(MLB_EINVAL, "%s: the plan has %lld partial rows but no workspace", what,
                 static_cast<long long>(num_partial_rows));
   if (!aligned(k_cache, 16) || !aligned(v_cache, 16)) return fail(MLB_EINVAL, "%s: pools must be 16-byte aligned", what);
+  // offsets into a pool are 32-bit counts of 16 bytes: up to 64 GiB a pool
+  if (num_blocks > (int64_t(1) << 32) / (static_cast<int64_t>(num_kv_heads) * 17 * head_dim / 32))
+    return fail(MLB_EUNSUPPORTED, "%s: a pool of more than 64 GiB", what);
   if (num_units > INT32_MAX / num_kv_heads || num_shared_units > INT32_MAX / num_kv_heads)
     return fail(MLB_EINVAL, "%s: grid too large", what);
   mlb::AttnArgs a{};
@@ -993,3 +1050,23 @@ int mlb_paged_attention_fp4(const void* q, int64_t q_stride_tok, int64_t q_strid
 }
 
 }  // extern "C"
+
+extern "C" int mlb_splitk_reduce_wide(const float* partial_o, const float* partial_lse, int64_t num_partial_rows,
+                                      const int32_t* reduce_rows, const int32_t* reduce_chunks, int tokens_per_tile_,
+                                      int64_t num_tokens, int num_heads, int head_dim, void* out,
+                                      int64_t out_stride_tok, int64_t out_stride_head, int out_dtype,
+                                      const mlb_out_targets* out_targets, void* stream) {
+  const char* what = "splitk_reduce_wide";
+  if (!elt_bytes(out_dtype)) return fail(MLB_EINVAL, "%s: unknown dtype %d", what, out_dtype);
+  if (!fp4_head_dim(head_dim)) return fail(MLB_EUNSUPPORTED, "%s: head_dim %d", what, head_dim);
+  if (num_tokens < 0 || num_heads <= 0 || tokens_per_tile_ <= 0) return fail(MLB_EINVAL, "%s: bad sizes", what);
+  if (num_tokens == 0 || num_partial_rows == 0) return MLB_OK;
+  if (num_tokens > INT32_MAX / num_heads) return fail(MLB_EINVAL, "%s: grid too large", what);
+  if (!partial_o || !partial_lse || !reduce_rows || !reduce_chunks) return fail(MLB_EINVAL, "%s: null pointer", what);
+  mlb_out_targets targets;
+  if (int rc = resolve_targets(what, out, out_stride_tok, out_stride_head, out_targets, &targets)) return rc;
+  return cuda_status(mlb::launch_splitk_reduce_wide(partial_o, partial_lse, reduce_rows, reduce_chunks, tokens_per_tile_,
+                                                    num_tokens, num_heads, head_dim, targets, out_dtype,
+                                                    static_cast<cudaStream_t>(stream)),
+                     what);
+}

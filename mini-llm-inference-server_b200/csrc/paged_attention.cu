@@ -712,6 +712,70 @@ __global__ void __launch_bounds__(256) splitk_reduce_kernel(const float* po, con
   store_out_n<OUT_DT, DPL>(out, out_vec != 0, tok, head, lane * DPL, acc);
 }
 
+// The same for few tokens of many pieces (one long row on the whole GPU): one CTA per (token, query head), its 8
+// warps taking the pieces round robin, so a row of 74 pieces is two rounds of loads instead of 19.
+constexpr int kWideWarps = 8;
+
+template <int DH, int OUT_DT>
+__global__ void __launch_bounds__(kWideWarps * 32) splitk_reduce_wide_kernel(const float* po, const float* plse,
+                                                                            const int32_t* rrows,
+                                                                            const int32_t* rchunks, int tpt, int h,
+                                                                            const mlb_out_targets out, int out_vec) {
+  constexpr int DPL = DH / 32, BATCH = 5;
+  __shared__ float sacc[kWideWarps][DH], slw[kWideWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t tok = blockIdx.x / h;
+  const int head = static_cast<int>(blockIdx.x % h);
+  const int nc = rchunks[tok];  // the plan's arrays: read before the wait, as above
+  const int64_t r0 = rrows[tok];
+  griddep_begin();
+  if (nc <= 1) return;
+  auto at = [&](int c) { return (r0 + static_cast<int64_t>(c) * tpt) * h + head; };
+  float M = kNegInf;
+  for (int c = lane; c < nc; c += 32) M = fmaxf(M, plse[at(c)]);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+  float acc[DPL] = {}, lw = 0.f;
+  for (int c0 = warp; c0 < nc; c0 += kWideWarps * BATCH) {
+    float x[BATCH][DPL], lse[BATCH];
+#pragma unroll
+    for (int j = 0; j < BATCH; ++j) {
+      const int c = c0 + j * kWideWarps;
+      lse[j] = kNegInf;
+      if (c < nc) {
+        lse[j] = plse[at(c)];
+        load_f32<DPL>(po + at(c) * DH + lane * DPL, x[j]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < BATCH; ++j) {
+      if (lse[j] == kNegInf) continue;  // no such piece, or one that saw no key
+      const float w = fast_exp2(lse[j] - M);
+      lw += w;
+#pragma unroll
+      for (int i = 0; i < DPL; ++i) acc[i] = fmaf(w, x[j][i], acc[i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < DPL; ++i) sacc[warp][lane * DPL + i] = acc[i];
+  if (lane == 0) slw[warp] = lw;
+  __syncthreads();
+  if (warp) return;
+  lw = 0.f;
+#pragma unroll
+  for (int i = 0; i < DPL; ++i) acc[i] = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWideWarps; ++w) {
+    lw += slw[w];
+#pragma unroll
+    for (int i = 0; i < DPL; ++i) acc[i] += sacc[w][lane * DPL + i];
+  }
+  const float inv = lw == 0.f ? 0.f : 1.f / lw;
+#pragma unroll
+  for (int i = 0; i < DPL; ++i) acc[i] *= inv;
+  store_out_n<OUT_DT, DPL>(out, out_vec != 0, tok, head, lane * DPL, acc);
+}
+
 // The split-K reduction carrying the output all-gather: one warp per (token, query head) of this rank.
 // Split tokens are reduced into every destination; unsplit tokens' rows (written by the attention kernel
 // into destination `self` only) are copied from there to the others.  No fence here: the barrier kernel
@@ -946,6 +1010,21 @@ cudaError_t launch_splitk_reduce(const float* po, const float* plse, const int32
   MLB_RED(128, MLB_F32) MLB_RED(128, MLB_F16) MLB_RED(128, MLB_BF16)
   MLB_RED(256, MLB_F32) MLB_RED(256, MLB_F16) MLB_RED(256, MLB_BF16)
 #undef MLB_RED
+  return cudaErrorInvalidValue;
+}
+
+cudaError_t launch_splitk_reduce_wide(const float* po, const float* plse, const int32_t* rrows, const int32_t* rchunks,
+                                      int tpt, int64_t ntok, int h, int dh, const mlb_out_targets& out, int out_dtype,
+                                      cudaStream_t s) {
+  const int vec = out_vec_ok(out, out_dtype == MLB_F32 ? 4 : 2) ? 1 : 0;
+#define MLB_REDW(D, O)                                                                                              \
+  if (dh == D && out_dtype == O)                                                                                    \
+    return launch_k(splitk_reduce_wide_kernel<D, O>, dim3(static_cast<unsigned>(ntok * h)), dim3(kWideWarps * 32), 0, \
+                    s, po, plse, rrows, rchunks, tpt, h, out, vec);
+  MLB_REDW(64, MLB_F32) MLB_REDW(64, MLB_F16) MLB_REDW(64, MLB_BF16)
+  MLB_REDW(128, MLB_F32) MLB_REDW(128, MLB_F16) MLB_REDW(128, MLB_BF16)
+  MLB_REDW(256, MLB_F32) MLB_REDW(256, MLB_F16) MLB_REDW(256, MLB_BF16)
+#undef MLB_REDW
   return cudaErrorInvalidValue;
 }
 

@@ -116,6 +116,7 @@ class AttentionPlan:
     reduce_rows_host: np.ndarray
     reduce_chunks_host: np.ndarray  # [N] pieces per token on the host
     has_query_tiles: bool = False  # kind-1 shared units (rows of >= 16 new tokens) in the plan
+    max_pieces: int = 0  # the most pieces of one token
 
 
 def _i32(a) -> np.ndarray:
@@ -145,6 +146,8 @@ def plan_attention(qo_indptr: list[int], seq_lens: list[int], max_blocks: int, n
     tables = None if block_tables_host is None else _i32(block_tables_host)
     if tables is not None and (tables.ndim != 2 or tables.shape[0] != s):
         raise ValueError(f"plan: block_tables_host must be [{s}, W], got {tables.shape}")
+    if pool_dtype is torch.uint8 and pages_per_unit <= 0:
+        pages_per_unit = _lib.PAGES_PER_UNIT_FP4
     L = lib()
     nu, ns, nm, npart = (ctypes.c_int64(0) for _ in range(4))
     head = (qo.ctypes.data, lens.ctypes.data, s, max_blocks, None if tables is None else tables.ctypes.data,
@@ -171,7 +174,8 @@ def plan_attention(qo_indptr: list[int], seq_lens: list[int], max_blocks: int, n
                          seg[2].view(m, MEMBER_INT32S), seg[3], seg[4], npart.value,
                          max(1, 8 // (num_heads // num_kv_heads)), num_heads, num_kv_heads, n_tok,
                          units[:u].copy(), shared[:sh].copy(), members[:m].copy(), rows[:n_tok].copy(),
-                         chunks[:n_tok].copy(), bool(sh and ((shared[:sh, 6] & 0xFF) == 1).any()))
+                         chunks[:n_tok].copy(), bool(sh and ((shared[:sh, 6] & 0xFF) == 1).any()),
+                         int(chunks[:n_tok].max()) if n_tok else 0)
 
 
 class Workspace:
@@ -304,9 +308,10 @@ def can_fuse_append(plan: AttentionPlan, k_cache: torch.Tensor, k: torch.Tensor,
 
 def splitk_reduce(plan: AttentionPlan, workspace: Workspace, out: torch.Tensor | None,
                   targets: OutTargets | None = None, dtype: torch.dtype | None = None, head_dim: int | None = None,
-                  device: torch.device | None = None) -> None:
+                  device: torch.device | None = None, wide: bool = False) -> None:
     """K2b: combine the split sequences' partial rows into `out` (no-op when the plan split nothing).
-    With `targets`, the rows go there instead; dtype / head_dim / device then describe them."""
+    With `targets`, the rows go there instead; dtype / head_dim / device then describe them.  `wide` shares a
+    token's pieces between the warps of a CTA (few tokens of many pieces)."""
     if not plan.num_partial_rows or plan.num_tokens == 0:
         return
     if targets is None:
@@ -315,9 +320,10 @@ def splitk_reduce(plan: AttentionPlan, workspace: Workspace, out: torch.Tensor |
         dtype, head_dim, device = out.dtype, out.shape[2], out.device
     n, h = plan.num_tokens, plan.num_heads
     po, plse = workspace.get(plan.num_partial_rows, h, head_dim, device)
-    rc = lib().mlb_splitk_reduce(po.data_ptr(), plse.data_ptr(), plan.num_partial_rows, plan.reduce_rows.data_ptr(),
-                                 plan.reduce_chunks.data_ptr(), plan.tokens_per_tile, n, h, head_dim, _ptr(out),
-                                 *_strides(out), DTYPE_CODE[dtype], _targets(targets), _stream(device))
+    reduce = lib().mlb_splitk_reduce_wide if wide else lib().mlb_splitk_reduce
+    rc = reduce(po.data_ptr(), plse.data_ptr(), plan.num_partial_rows, plan.reduce_rows.data_ptr(),
+                plan.reduce_chunks.data_ptr(), plan.tokens_per_tile, n, h, head_dim, _ptr(out), *_strides(out),
+                DTYPE_CODE[dtype], _targets(targets), _stream(device))
     check(rc, "splitk_reduce")
 
 
@@ -367,6 +373,7 @@ def _targets(t: OutTargets | None):
 
 FP4_ROWS = BLOCK_SIZE + 1  # rows of a (block, head): 16 tokens' codes, then their scales
 FP4_RUN = 32  # dims that share a scale
+WIDE_REDUCE_PIECES = 8  # rows of more pieces than this are reduced by a CTA per head instead of a warp
 
 
 def is_fp4(pool: torch.Tensor) -> bool:
@@ -511,7 +518,8 @@ def paged_attention_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     out = attention_partials_fp4(q, k_cache, v_cache, block_tables, seq_lens, qo_indptr, plan, workspace, out, scale,
                                  err, targets)
     with _on(q.device):
-        splitk_reduce(plan, workspace, out, targets, q.dtype, q.shape[2], q.device)
+        splitk_reduce(plan, workspace, out, targets, q.dtype, q.shape[2], q.device,
+                      wide=plan.max_pieces > WIDE_REDUCE_PIECES)
     return out
 
 
