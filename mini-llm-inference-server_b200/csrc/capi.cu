@@ -43,6 +43,8 @@ cudaError_t launch_fp4_append(const RowArgs& a, int dtype, int dh, int num_sms, 
 cudaError_t launch_fp4_read(const RowArgs& a, int dtype, int dh, int num_sms, cudaStream_t s);
 cudaError_t launch_fp4_attention(const AttnArgs& a, int dtype, int dh, int64_t num_units, cudaStream_t s);
 cudaError_t launch_fp4_shared(const AttnArgs& a, int dtype, int dh, int64_t num_units, cudaStream_t s);
+bool fp4_shared_tc_supported(const AttnArgs& a, int dh);
+cudaError_t launch_fp4_shared_tc(const AttnArgs& a, int dtype, int dh, int64_t num_units, cudaStream_t s);
 cudaError_t launch_block_copy(void* const* pools, int num_pools, int64_t num_blocks, int64_t block_bytes,
                               const int32_t* src, const int32_t* dst, int64_t num_pairs, int32_t* err, int num_sms,
                               cudaStream_t s);
@@ -88,6 +90,7 @@ constexpr int kSharedCtasPerSm = 1;  // resident shared-prefix CTAs per SM (the 
 #define MLB_TILE_PAGE_HEADS 19
 #endif
 constexpr int kTilePageHeads = MLB_TILE_PAGE_HEADS;
+constexpr int kFp4TilePageHeads = 40;  // the same against a 4-bit page-head (~0.05 us)
 constexpr int kMinSharedSmPct = 25;  // the shared-prefix kernel gets at least this share of the SMs
 constexpr int kMinShareSeqs = 4;     // a shared prefix is planned once only for this many decode rows ...
 constexpr int kMinSharePages = 8;    // ... sharing at least this many full pages
@@ -391,6 +394,7 @@ int mlb_plan_attention(const int32_t* qo_indptr, const int32_t* seq_lens, int nu
   for (const Group& g : groups) rest += g.pages - g.start;
   // The shared-prefix kernel runs beside the per-sequence kernel, one CTA per SM: it gets the share of the
   // SMs that balances the two kernels' estimated SM time (all of them when no per-sequence work is left)
+  const int64_t tile_cost = pages_per_unit == MLB_PAGES_PER_UNIT_FP4 ? kFp4TilePageHeads : kTilePageHeads;
   int64_t tc_work = 0;
   // a tensor-core CTA takes one member block of a shared prefix (its single-tile pipeline double-buffers S,
   // which measured faster there than two blocks per CTA)
@@ -398,8 +402,7 @@ int mlb_plan_attention(const int32_t* qo_indptr, const int32_t* seq_lens, int nu
     return (static_cast<int64_t>(set.seqs.size()) + per_cta - 1) / per_cta;
   };
   for (const ShareSet& set : sets)
-    tc_work += blocks_of(set) * num_kv_heads * ((set.pages + kMinPagesPerUnit - 1) / kMinPagesPerUnit) *
-               kTilePageHeads;
+    tc_work += blocks_of(set) * num_kv_heads * ((set.pages + kMinPagesPerUnit - 1) / kMinPagesPerUnit) * tile_cost;
   const int64_t priv_work = rest * num_kv_heads;
   const int64_t share_pct =
       tc_work > 0 ? std::max<int64_t>(kMinSharedSmPct, 100 * tc_work / (tc_work + priv_work)) : 100;
@@ -594,6 +597,37 @@ int mlb_plan_attention(const int32_t* qo_indptr, const int32_t* seq_lens, int nu
 
 namespace {
 
+// Launch a plan's shared units (launch_shared) and its per-sequence units (launch_rows) on stream `st`.
+template <typename Shared, typename Rows>
+int run_shared_and_rows(const char* what, int64_t num_shared_units, int64_t num_units, cudaStream_t st,
+                        Shared launch_shared, Rows launch_rows) {
+  if (num_shared_units > 0 && num_units > 0 && mlb::concurrent_prefix()) {
+    // The two kernels write disjoint rows and neither reads what the other writes (a page written by the
+    // fused append is private to its row, never part of a shared unit): fork the shared-prefix kernel onto
+    // a high-priority side stream (its CTAs, one per SM, are placed first), run the per-sequence kernel
+    // beside it on the caller's stream (it fills the free SMs and the shared kernel's tail), and join, so
+    // whatever the caller queues next (the split-K reduction) waits for both.  Captures into CUDA graphs
+    // as a fork and a join.
+    SideStream* ss = nullptr;
+    cudaError_t e = side_stream(&ss);
+    if (e == cudaSuccess) e = cudaEventRecord(ss->fork, st);
+    if (e == cudaSuccess) e = cudaStreamWaitEvent(ss->stream, ss->fork, 0);
+    if (e != cudaSuccess) return cuda_status(e, what);
+    cudaError_t el = launch_shared(ss->stream);
+    if (el == cudaSuccess) el = launch_rows(st);
+    // joined whatever happened above, so a stream capture never ends with the side stream still forked
+    cudaError_t ej = cudaEventRecord(ss->join, ss->stream);
+    if (ej == cudaSuccess) ej = cudaStreamWaitEvent(st, ss->join, 0);
+    return cuda_status(el != cudaSuccess ? el : ej, what);
+  }
+  if (num_shared_units > 0) {
+    const int rc = cuda_status(launch_shared(st), what);
+    if (rc != MLB_OK) return rc;
+  }
+  if (num_units == 0) return MLB_OK;
+  return cuda_status(launch_rows(st), what);
+}
+
 // mlb_paged_attention and mlb_paged_attention_append: `app` (validated by the caller) or nullptr.
 int attention_call(const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k_cache,
                    const void* v_cache, int dtype, int64_t num_blocks, int block_size, int num_heads,
@@ -674,31 +708,9 @@ int attention_call(const void* q, int64_t q_stride_tok, int64_t q_stride_head, c
     return tc ? mlb::launch_shared_prefix_tc(a, dtype, head_dim, num_shared_units, s)
               : mlb::launch_shared_prefix_attention(a, dtype, head_dim, num_shared_units, s);
   };
-  if (num_shared_units > 0 && num_units > 0 && mlb::concurrent_prefix()) {
-    // The two kernels write disjoint rows and neither reads what the other writes (a page written by the
-    // fused append is private to its row, never part of a shared unit): fork the shared-prefix kernel onto
-    // a high-priority side stream (its CTAs, one per SM, are placed first), run the per-sequence kernel
-    // beside it on the caller's stream (it fills the free SMs and the shared kernel's tail), and join, so
-    // whatever the caller queues next (the split-K reduction) waits for both.  Captures into CUDA graphs
-    // as a fork and a join.
-    SideStream* ss = nullptr;
-    cudaError_t e = side_stream(&ss);
-    if (e == cudaSuccess) e = cudaEventRecord(ss->fork, st);
-    if (e == cudaSuccess) e = cudaStreamWaitEvent(ss->stream, ss->fork, 0);
-    if (e != cudaSuccess) return cuda_status(e, "paged_attention: side stream fork");
-    cudaError_t el = launch_shared(ss->stream);
-    if (el == cudaSuccess) el = mlb::launch_paged_attention(a, dtype, head_dim, num_units, st);
-    // joined whatever happened above, so a stream capture never ends with the side stream still forked
-    cudaError_t ej = cudaEventRecord(ss->join, ss->stream);
-    if (ej == cudaSuccess) ej = cudaStreamWaitEvent(st, ss->join, 0);
-    return cuda_status(el != cudaSuccess ? el : ej, "paged_attention launch (shared-prefix kernel on a side stream)");
-  }
-  if (num_shared_units > 0) {
-    const int rc = cuda_status(launch_shared(st), "shared-prefix attention launch");
-    if (rc != MLB_OK) return rc;
-  }
-  if (num_units == 0) return MLB_OK;
-  return cuda_status(mlb::launch_paged_attention(a, dtype, head_dim, num_units, st), "paged_attention launch");
+  return run_shared_and_rows(
+      "paged_attention", num_shared_units, num_units, st, launch_shared,
+      [&](cudaStream_t s) { return mlb::launch_paged_attention(a, dtype, head_dim, num_units, s); });
 }
 
 }  // namespace
@@ -1042,11 +1054,14 @@ int mlb_paged_attention_fp4(const void* q, int64_t q_stride_tok, int64_t q_strid
   a.q_vec = rows_aligned(q, q_stride_tok, q_stride_head, 2) ? 1 : 0;
   a.err = err_word;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (num_shared_units > 0) {
-    const int rc = cuda_status(mlb::launch_fp4_shared(a, dtype, head_dim, num_shared_units, st), what);
-    if (rc != MLB_OK || num_units == 0) return rc;
-  }
-  return cuda_status(mlb::launch_fp4_attention(a, dtype, head_dim, num_units, st), what);
+  const bool tc = num_shared_units > 0 && mlb::tensor_core_prefix() && mlb::fp4_shared_tc_supported(a, head_dim);
+  return run_shared_and_rows(
+      what, num_shared_units, num_units, st,
+      [&](cudaStream_t s) {
+        return tc ? mlb::launch_fp4_shared_tc(a, dtype, head_dim, num_shared_units, s)
+                  : mlb::launch_fp4_shared(a, dtype, head_dim, num_shared_units, s);
+      },
+      [&](cudaStream_t s) { return mlb::launch_fp4_attention(a, dtype, head_dim, num_units, s); });
 }
 
 }  // extern "C"

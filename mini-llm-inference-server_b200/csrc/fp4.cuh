@@ -88,4 +88,12 @@ __device__ __forceinline__ float fp4_quotient(float x, float scale, float inv) {
   return copysignf(q, x);  // the correction would turn -0 into +0
 }
 
+// bf16 query rows enter fp16 products divided by the power of two of their largest element mx: down = 2^-e, up = 2^e,
+// with e kept where both are normal numbers.
+__device__ __forceinline__ void fp4_query_scale(float mx, float& up, float& down) {
+  const int e = max(1, min(static_cast<int>(__float_as_uint(mx) >> 23), 253));  // biased exponent
+  down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+  up = __uint_as_float(static_cast<uint32_t>(e) << 23);
+}
+
 }  // namespace mlb

@@ -137,10 +137,8 @@ __device__ __forceinline__ void load_queries(Columns<DH>& c, const AttnArgs& a, 
     }
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-    // biased exponent of the row's largest element, kept where both powers of two are normal numbers
-    const int e = max(1, min(static_cast<int>(__float_as_uint(mx) >> 23), 253));
-    const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);  // 2^(127 - e)
-    f = __uint_as_float(static_cast<uint32_t>(e) << 23);                       // 2^(e - 127)
+    float down;
+    fp4_query_scale(mx, f, down);
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) {
       const uint32_t w = c.qb[i >> 1][i & 1];

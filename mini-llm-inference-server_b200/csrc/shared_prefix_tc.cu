@@ -36,6 +36,13 @@
 // TMEM columns, paired: S_A [0,128), S_B [128,256), O_A [256, 256 + Dh), O_B [256 + Dh, 256 + 2 Dh);
 // single: S buffers [0,128), [128,256), [256,384), O [384, 384 + Dh).
 //
+// 4-bit pools (FP4; fp4.cuh) take the same kernel with other feeders: 512 threads, warps 12-15 load each tile's codes
+// (thread = key row, one tile ahead, in registers), widen them to fp16 (code * scale, exact) and store them where
+// TMA would have put them; rows that must not be seen (a bad block id, past the sequence's end) are stored as
+// zeros, so nothing is cleared later.  About 160 instructions a thread and tile of 128 x 128, a fifth of a tile's
+// time beside the softmax.  Q and P are fp16 for both output types: a bf16 query row is divided by the power of
+// two of its largest element (exact), which goes into the row's softmax scale.
+//
 // Every wait is bounded (time and polls); on expiry the CTA raises MLB_DEV_WAIT_TIMEOUT, drains its own
 // copies and MMAs, frees TMEM and returns.
 #include <cuda.h>
@@ -47,21 +54,29 @@
 #include <unordered_map>
 
 #include "attn_args.cuh"
+#include "fp4.cuh"
 #include "tcgen05.cuh"
 
 namespace mlb {
 
 namespace {
 
-constexpr int kTcThreads = 384;     // 12 warps: 3 producers, the MMA issuer, two softmax warpgroups
+// 12 warps: 3 producers, the MMA issuer, two softmax warpgroups; 4-bit pools: the issuer's warpgroup, two softmax
+// warpgroups and one that widens codes
+template <bool FP4>
+constexpr int kTcThreads = FP4 ? 512 : 384;
 constexpr int kTcRows = 128;        // query columns per tile = MMA M = TMEM lanes
 constexpr int kTcTileTokens = 128;  // keys per tile = N of S = Q . K^T
 constexpr int kTcTilePages = kTcTileTokens / kBlockSize;
 constexpr uint32_t kTmemCols = 512;
-// registers per thread: at launch (384 threads on one SM), after the split for warps 0-3 and for the softmax
-constexpr int kRegsLaunch = 168, kRegsLow = 56, kRegsHigh = 224;
-static_assert(128 * (kRegsLaunch - kRegsLow) == 256 * (kRegsHigh - kRegsLaunch), "the split must balance");
-static_assert(kRegsLaunch * kTcThreads <= 65536, "one CTA per SM");
+// registers per thread: at launch (384 or 512 threads on one SM), after the split for warps 0-3, for the softmax and
+// for the warps that widen codes
+template <bool FP4>
+struct TcRegs {
+  static constexpr int kLaunch = FP4 ? 128 : 168, kLow = FP4 ? 40 : 56, kHigh = FP4 ? 208 : 224, kFeed = FP4 ? 56 : 0;
+  static_assert(128 * kLow + 256 * kHigh + 128 * kFeed == kLaunch * kTcThreads<FP4>, "the split must balance");
+  static_assert(kLaunch * kTcThreads<FP4> <= 65536, "one CTA per SM");
+};
 // TMEM columns: S_A [0,128), S_B [128,256), O_A [256, 256 + Dh), O_B after it; P_x (16-bit pairs) over the
 // first 64 columns of S_x
 __device__ __forceinline__ uint32_t col_s(int x) { return x ? 128u : 0u; }
@@ -95,13 +110,55 @@ __device__ __forceinline__ uint32_t sw_chunk(int r, int c) {
   return static_cast<uint32_t>((c >> 3) * (kTcRows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
-template <int DT, int DH>
-__global__ void __launch_bounds__(kTcThreads, 1) shared_prefix_tc_kernel(AttnArgs a, const __grid_constant__ CUtensorMap tk,
-                                                                          const __grid_constant__ CUtensorMap tv) {
+// What a feeder thread holds of a tile: its key's codes and scale bytes.
+template <int DH>
+struct FeedRow {
+  uint32_t w[DH / 8];
+  uint32_t scales[DH / 128 > 0 ? DH / 128 : 1];  // a byte for each run of 32 dims
+  __device__ __forceinline__ void load(const uint8_t* rec, int t) {  // rec == nullptr: a key that reads as zeros
+    constexpr int RUNS = DH / kFp4Run;
+    if (rec) {
+      const uint4* src = reinterpret_cast<const uint4*>(rec + t * Fp4<DH>::kRow);
+#pragma unroll
+      for (int i = 0; i < DH / 32; ++i) {
+        const uint4 x = __ldg(src + i);
+        w[4 * i] = x.x, w[4 * i + 1] = x.y, w[4 * i + 2] = x.z, w[4 * i + 3] = x.w;
+      }
+      uint32_t b = 0;
+#pragma unroll
+      for (int r = 0; r < RUNS; ++r)
+        b |= static_cast<uint32_t>(__ldg(rec + Fp4<DH>::kScales + fp4_scale_at(r, t))) << (8 * r);
+      scales[0] = b;
+    } else {
+#pragma unroll
+      for (int i = 0; i < DH / 8; ++i) w[i] = 0u;
+      scales[0] = 0u;
+    }
+  }
+  // row `row` of a [DH/64][128][64] swizzled fp16 tile
+  __device__ __forceinline__ void store(uint32_t tile, int row) const {
+#pragma unroll
+    for (int c = 0; c < DH / 8; ++c) {
+      const uint32_t s = ((scales[0] >> (8 * (c / 4))) & 0xffu) * 0x00010001u << 7;
+      uint32_t x[4];
+      fp4_unpack8(w[c], x[0], x[1], x[2], x[3]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = hmul2_u32(x[i], s);
+      asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(tile + sw_chunk(row, c)), "r"(x[0]), "r"(x[1]),
+                   "r"(x[2]), "r"(x[3])
+                   : "memory");
+    }
+  }
+};
+
+template <int DT, int DH, bool FP4>
+__global__ void __launch_bounds__(kTcThreads<FP4>, 1)
+    shared_prefix_tc_kernel(AttnArgs a, const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv) {
   using L = TcLayout<DH>;
   constexpr int NK = L::kKStages, NV = L::kVStages;
   constexpr int CH = DH * 2 / 16;  // 16-byte chunks per row
-  constexpr uint32_t kFmt = DT == MLB_BF16 ? 1u : 0u;
+  constexpr int MT = FP4 ? MLB_F16 : DT;  // type of the products' operands
+  constexpr uint32_t kFmt = MT == MLB_BF16 ? 1u : 0u;
   constexpr uint32_t kIdescS = f16_idesc(kFmt, false, kTcRows, kTcTileTokens);
   constexpr uint32_t kIdescO = f16_idesc(kFmt, true, kTcRows, DH);
   constexpr float kNegInfF = -__builtin_huge_valf();
@@ -144,11 +201,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_prefix_tc_kernel(AttnArg
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < NK; ++s) {
-      mbar_init(kfull + s, 1);
+      mbar_init(kfull + s, FP4 ? 128 : 1);
       mbar_init(kempty + s, 1);
     }
     for (int s = 0; s < NV; ++s) {
-      mbar_init(vfull + s, 1);
+      mbar_init(vfull + s, FP4 ? 128 : 1);
       mbar_init(vempty + s, 1);
     }
     for (int b = 0; b < 3; ++b) {
@@ -172,19 +229,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_prefix_tc_kernel(AttnArg
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  // Register split: the producer / MMA warpgroup (warps 0-3) drops to kRegsLow, the two softmax warpgroups
-  // take what it frees (kRegsHigh each).  The launch gives every thread kRegsLaunch (checked on the host
-  // against the compiled kernel before any launch), so 128 x (launch - low) = 256 x (high - launch) exactly.
+  // Register split: the producer / MMA warpgroup (warps 0-3) drops to kLow (and the 4-bit feeders to kFeed), the two
+  // softmax warpgroups take what they free (kHigh each).  The launch gives every thread kLaunch (checked on the host
+  // against the compiled kernel before any launch), so the shares add up to the launch's exactly.
   if (warp < 4) {
     // warpgroup 0 gives up registers, all four warps at the same instruction
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLow));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TcRegs<FP4>::kLow));
     if (warp != 1) {
       // ------------------------------------------------------------ producers: warp 0 fills the K ring,
       // warp 2 the V ring (warp 3 has no role), so a K tile never queues behind a V slot: the K ring runs up
       // to kKStages tiles ahead of the scores while V stages wait for their P . V products.  Lane p loads
       // page p's block id one tile ahead (the table round trip overlaps the previous tile) and issues the
       // page's Dh/64 boxes; lane 0 declares the tile's bytes on the stage barrier (one arrival per phase).
-      if (warp != 3) {
+      if (!FP4 && warp != 3) {
         constexpr uint32_t kBoxBytes = 64 * 2 * kBlockSize;  // {64 dims, 1 head, 16 slots}
         constexpr int kHalves = DH / 64;
         const bool is_v = warp == 2;
@@ -329,8 +386,48 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_prefix_tc_kernel(AttnArg
         if (!tc_drain(final_bar, 0)) flag_error(a.err, MLB_DEV_WAIT_TIMEOUT);
       }
     }
+  } else if (FP4 && warp >= 12) {
+    if constexpr (FP4) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TcRegs<FP4>::kFeed));
+      // ---------------------------------------------------------- feeders: thread = key row of every tile.  A row's
+      // loads are issued a tile ahead of its stores, K's while V is stored and the other way round.
+      const int row = threadIdx.x - 384, page_in = row / kBlockSize, t = row % kBlockSize;
+      const int64_t block_bytes = static_cast<int64_t>(a.hkv) * Fp4<DH>::kRecord;
+      const int64_t head_off = static_cast<int64_t>(kvh) * Fp4<DH>::kRecord;
+      const int seq_len = tile_unit ? __ldg(a.seq_lens + tseq) : INT_MAX;
+      auto offset = [&](int j) -> int64_t {  // of the row's page in a pool; -1: nothing to see
+        const int page = j * kTcTilePages + page_in;
+        if (j >= ntiles || page >= npages) return -1;
+        const int bid = __ldg(table + pb + page);
+        if (bid < 0 || bid >= a.num_blocks) {
+          if (t == 0) flag_error(a.err, MLB_DEV_BLOCK_RANGE);
+          return -1;
+        }
+        if ((pb + page) * kBlockSize + t >= seq_len) return -1;
+        return bid * block_bytes + head_off;
+      };
+      const uint8_t* kp = reinterpret_cast<const uint8_t*>(a.k_cache);
+      const uint8_t* vp = reinterpret_cast<const uint8_t*>(a.v_cache);
+      FeedRow<DH> k, v;
+      int64_t off = offset(0);
+      k.load(off < 0 ? nullptr : kp + off, t);
+      v.load(off < 0 ? nullptr : vp + off, t);
+      for (int j = 0; j < ntiles; ++j) {
+        const int64_t next = offset(j + 1);
+        if (j >= NK && !tc_wait(kempty + j % NK, ((j / NK) + 1) & 1, abort_flag, a.err)) break;
+        k.store(k_smem + (j % NK) * L::kTileBytes, row);
+        fence_proxy_async_smem();  // generic-proxy stores, read by the tensor core (async proxy)
+        mbar_arrive(kfull + j % NK);
+        k.load(next < 0 ? nullptr : kp + next, t);
+        if (j >= NV && !tc_wait(vempty + j % NV, ((j / NV) + 1) & 1, abort_flag, a.err)) break;
+        v.store(v_smem + (j % NV) * L::kTileBytes, row);
+        fence_proxy_async_smem();
+        mbar_arrive(vfull + j % NV);
+        v.load(next < 0 ? nullptr : vp + next, t);
+      }
+    }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsHigh));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TcRegs<FP4>::kHigh));
     // ------------------------------------------------------------ softmax warpgroups: warps 4-7 take tile A,
     // warps 8-11 tile B; one thread = one query column = one TMEM lane
     const int x = warp >= 8 ? 1 : 0;
@@ -339,6 +436,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_prefix_tc_kernel(AttnArg
     const int tile_pieces = (x ? yb.z : ya.z) >> 8, tile_part_base = x ? yb.w : ya.w;
     // the Q rows first, straight into the swizzled K-major A tile (zero for absent columns); the producers
     // are already fetching the first K/V tiles, and only the MMA issuer waits for q_ready
+    float sl2 = a.sl2;
     {
       const int m = row / a.group;
       const bool live = m < mc && (x == 0 || two);
@@ -350,10 +448,35 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_prefix_tc_kernel(AttnArg
             a.q + (static_cast<int64_t>(tok) * a.q_st + static_cast<int64_t>(head) * a.q_sh) * 2);
       }
       uint8_t* qx = smem + x * L::kQBytes;
+      if constexpr (FP4 && DT == MLB_BF16) {
+        uint32_t w[4 * CH];
+        float mx = 0.f;
 #pragma unroll
-      for (int ch = 0; ch < CH; ++ch) {
-        const uint4 v = live ? __ldg(src + ch) : make_uint4(0u, 0u, 0u, 0u);
-        *reinterpret_cast<uint4*>(qx + sw_chunk(row, ch)) = v;
+        for (int ch = 0; ch < CH; ++ch) {
+          const uint4 v = live ? __ldg(src + ch) : make_uint4(0u, 0u, 0u, 0u);
+          w[4 * ch] = v.x, w[4 * ch + 1] = v.y, w[4 * ch + 2] = v.z, w[4 * ch + 3] = v.w;
+        }
+#pragma unroll
+        for (int i = 0; i < 4 * CH; ++i)
+          mx = fmaxf(mx, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u))));
+        float up, down;
+        fp4_query_scale(mx, up, down);
+        sl2 *= up;
+#pragma unroll
+        for (int ch = 0; ch < CH; ++ch) {
+          uint32_t h[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            h[i] = pack2<MLB_F16>(__uint_as_float(w[4 * ch + i] << 16) * down,
+                                  __uint_as_float(w[4 * ch + i] & 0xffff0000u) * down);
+          *reinterpret_cast<uint4*>(qx + sw_chunk(row, ch)) = make_uint4(h[0], h[1], h[2], h[3]);
+        }
+      } else {
+#pragma unroll
+        for (int ch = 0; ch < CH; ++ch) {
+          const uint4 v = live ? __ldg(src + ch) : make_uint4(0u, 0u, 0u, 0u);
+          *reinterpret_cast<uint4*>(qx + sw_chunk(row, ch)) = v;
+        }
       }
       fence_proxy_async_smem();  // generic-proxy stores, read by the tensor core (async proxy)
     }
@@ -428,7 +551,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_prefix_tc_kernel(AttnArg
       for (int k = 8; k < kTcTileTokens; ++k) mx8[k % 8] = fmaxf(mx8[k % 8], __uint_as_float(sr[k]));
       const float mraw = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])),
                                fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
-      if (tile_unit && x == 0) {
+      if (!FP4 && tile_unit && x == 0) {
         // V rows of slots past the sequence's end (its last page) are junk: 0 x NaN would poison P . V, so
         // they are zeroed in shared memory before the tile goes to the tensor core (tile A's threads do it
         // before they release P_A; the MMA issues P_B . V after P_A . V)
@@ -448,7 +571,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_prefix_tc_kernel(AttnArg
           fence_proxy_async_smem();
         }
       }
-      const float mx = mraw * a.sl2;  // the scale is positive: max commutes with it
+      const float mx = mraw * sl2;  // the scale is positive: max commutes with it
       const bool need = mx > m_used + 8.f;
       if (__any_sync(0xffffffffu, need)) {
         const float m_new = need ? fmaxf(m_used, mx) : m_used;
@@ -480,7 +603,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_prefix_tc_kernel(AttnArg
       // exponentials stay on the special-function unit.  4 pair sums = 8 independent sum chains.
       const float nbase = m_used == kNegInfF ? 0.f : -m_used;
       uint64_t sl2v, nbv, s4[4];
-      asm("mov.b64 %0, {%1, %1};" : "=l"(sl2v) : "f"(a.sl2));
+      asm("mov.b64 %0, {%1, %1};" : "=l"(sl2v) : "f"(sl2));
       asm("mov.b64 %0, {%1, %1};" : "=l"(nbv) : "f"(nbase));
 #pragma unroll
       for (int i = 0; i < 4; ++i) s4[i] = 0ull;  // +0.0f in both halves
@@ -497,7 +620,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_prefix_tc_kernel(AttnArg
           const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
           asm("mov.b64 %0, {%1, %2};" : "=l"(pv) : "f"(p0), "f"(p1));
           asm("add.f32x2 %0, %0, %1;" : "+l"(s4[(k / 2) % 4]) : "l"(pv));
-          pk[k / 2] = pack2<DT>(p0, p1);
+          pk[k / 2] = pack2<MT>(p0, p1);
         }
         tmem_st32(s_cols + 32 * h, pk);
       }
@@ -517,7 +640,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_prefix_tc_kernel(AttnArg
     // TMEM in one go (Dh / 32 loads, one wait), and the row's destination was worked out before the tiles
     if (active && ok && ntiles > 0 && wait_warp(final_bar, 0) && !*abort_flag) {
       tc_fence_after();
-      const float inv = l > 0.f ? 1.f / l : 0.f;
+      // 4-bit pools: a NaN query's NaN sum stays one (the 16-bit path writes zeros)
+      const bool some = FP4 ? l != 0.f : l > 0.f;
+      const float inv = some ? 1.f / l : 0.f;
       uint32_t orow[DH];
 #pragma unroll
       for (int i = 0; i < DH / 32; ++i) tmem_ld32(o_cols + 32 * i, orow + 32 * i);
@@ -538,7 +663,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_prefix_tc_kernel(AttnArg
         for (int k = 0; k < DH / 4; ++k)
           dst[k] = make_float4(__uint_as_float(orow[4 * k]) * inv, __uint_as_float(orow[4 * k + 1]) * inv,
                                __uint_as_float(orow[4 * k + 2]) * inv, __uint_as_float(orow[4 * k + 3]) * inv);
-        a.part_lse[out_slot] = l > 0.f ? m_used + log2f(l) : kNegInfF;
+        a.part_lse[out_slot] = some ? m_used + log2f(l) : kNegInfF;
       }
     }
   }
@@ -593,32 +718,34 @@ cudaError_t pool_tensor_map(CUtensorMap* out, const void* pool, int dtype, int64
   return cudaSuccess;
 }
 
-template <int DT, int DH>
+template <int DT, int DH, bool FP4>
 cudaError_t launch_tc(const AttnArgs& a, int64_t units, cudaStream_t s) {
   constexpr int bytes = TcLayout<DH>::kLaunchBytes;
   static_assert(bytes <= 232448, "shared memory budget of one sm_100 CTA");
   static unsigned long long done = 0;
-  auto k = shared_prefix_tc_kernel<DT, DH>;
+  auto k = shared_prefix_tc_kernel<DT, DH, FP4>;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (!(dev < 64 && (done >> dev) & 1ull)) {
     // the register split inside the kernel (setmaxnreg) balances only if every thread starts with exactly
-    // kRegsLaunch registers; a build that compiled to another count is refused instead of launched
+    // kLaunch registers; a build that compiled to another count is refused instead of launched
     cudaFuncAttributes fa{};
     e = cudaFuncGetAttributes(&fa, k);
     if (e != cudaSuccess) return e;
-    if (fa.numRegs != kRegsLaunch) return cudaErrorInvalidKernelImage;
+    if (fa.numRegs != TcRegs<FP4>::kLaunch) return cudaErrorInvalidKernelImage;
     e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return e;
     if (dev < 64) __atomic_fetch_or(&done, 1ull << dev, __ATOMIC_RELAXED);
   }
-  CUtensorMap tk, tv;
-  e = pool_tensor_map(&tk, a.k_cache, DT, a.num_blocks, a.hkv, DH);
-  if (e == cudaSuccess) e = pool_tensor_map(&tv, a.v_cache, DT, a.num_blocks, a.hkv, DH);
-  if (e != cudaSuccess) return e;
+  CUtensorMap tk{}, tv{};
+  if constexpr (!FP4) {
+    e = pool_tensor_map(&tk, a.k_cache, DT, a.num_blocks, a.hkv, DH);
+    if (e == cudaSuccess) e = pool_tensor_map(&tv, a.v_cache, DT, a.num_blocks, a.hkv, DH);
+    if (e != cudaSuccess) return e;
+  }
   // one CTA per pair of units (2i, 2i + 1) and KV head
-  return launch_k(k, dim3(static_cast<unsigned>(units / 2 * a.hkv)), dim3(kTcThreads), bytes, s, a, tk, tv);
+  return launch_k(k, dim3(static_cast<unsigned>(units / 2 * a.hkv)), dim3(kTcThreads<FP4>), bytes, s, a, tk, tv);
 }
 
 }  // namespace
@@ -633,11 +760,25 @@ bool shared_prefix_tc_supported(const AttnArgs& a, int dtype, int dh) {
 
 cudaError_t launch_shared_prefix_tc(const AttnArgs& a, int dtype, int dh, int64_t num_units, cudaStream_t s) {
   if (dtype == MLB_BF16) {
-    if (dh == 64) return launch_tc<MLB_BF16, 64>(a, num_units, s);
-    if (dh == 128) return launch_tc<MLB_BF16, 128>(a, num_units, s);
+    if (dh == 64) return launch_tc<MLB_BF16, 64, false>(a, num_units, s);
+    if (dh == 128) return launch_tc<MLB_BF16, 128, false>(a, num_units, s);
   } else if (dtype == MLB_F16) {
-    if (dh == 64) return launch_tc<MLB_F16, 64>(a, num_units, s);
-    if (dh == 128) return launch_tc<MLB_F16, 128>(a, num_units, s);
+    if (dh == 64) return launch_tc<MLB_F16, 64, false>(a, num_units, s);
+    if (dh == 128) return launch_tc<MLB_F16, 128, false>(a, num_units, s);
+  }
+  return cudaErrorInvalidValue;
+}
+
+// The same for 4-bit pools (dtype: q's).
+bool fp4_shared_tc_supported(const AttnArgs& a, int dh) { return (dh == 64 || dh == 128) && a.q_vec; }
+
+cudaError_t launch_fp4_shared_tc(const AttnArgs& a, int dtype, int dh, int64_t num_units, cudaStream_t s) {
+  if (dtype == MLB_BF16) {
+    if (dh == 64) return launch_tc<MLB_BF16, 64, true>(a, num_units, s);
+    if (dh == 128) return launch_tc<MLB_BF16, 128, true>(a, num_units, s);
+  } else if (dtype == MLB_F16) {
+    if (dh == 64) return launch_tc<MLB_F16, 64, true>(a, num_units, s);
+    if (dh == 128) return launch_tc<MLB_F16, 128, true>(a, num_units, s);
   }
   return cudaErrorInvalidValue;
 }
