@@ -90,7 +90,7 @@ constexpr int kSharedCtasPerSm = 1;  // resident shared-prefix CTAs per SM (the 
 #define MLB_TILE_PAGE_HEADS 19
 #endif
 constexpr int kTilePageHeads = MLB_TILE_PAGE_HEADS;
-constexpr int kFp4TilePageHeads = 40;  // the same against a 4-bit page-head (~0.05 us)
+constexpr int kFp4TilePageHeads = 40;  // the same against a 4-bit page-head (~2.1 us a tile, ~0.05 us a page-head)
 constexpr int kMinSharedSmPct = 25;  // the shared-prefix kernel gets at least this share of the SMs
 constexpr int kMinShareSeqs = 4;     // a shared prefix is planned once only for this many decode rows ...
 constexpr int kMinSharePages = 8;    // ... sharing at least this many full pages
@@ -398,6 +398,7 @@ int mlb_plan_attention(const int32_t* qo_indptr, const int32_t* seq_lens, int nu
   int64_t tc_work = 0;
   // a tensor-core CTA takes one member block of a shared prefix (its single-tile pipeline double-buffers S,
   // which measured faster there than two blocks per CTA)
+  // (4-bit pools too: 128 rows behind 512 blocks 55.2 us single, 55.7 in pairs)
   auto blocks_of = [&](const ShareSet& set) {
     return (static_cast<int64_t>(set.seqs.size()) + per_cta - 1) / per_cta;
   };
@@ -498,13 +499,26 @@ int mlb_plan_attention(const int32_t* qo_indptr, const int32_t* seq_lens, int nu
   // limit masks the few keys it does not see); a row's last odd tile gets an empty partner.
   std::vector<std::array<mlb_shared_unit, 2>> tile_pairs;
   const int tile_tokens = std::max(1, kSharedColumns / group_size);
+  int64_t piece_pages = kPrefillPiecePages;
+  if (pages_per_unit == MLB_PAGES_PER_UNIT_FP4) {
+    // every piece costs a start, and its tokens' fp32 partial rows written and read again: rows are cut only as far
+    // as it takes to give every SM about 3 CTAs (4 rows of 1500..2000 new tokens, 4-bit pools: 882 us in pieces of
+    // 128 pages, 668 us whole)
+    int64_t work = 0;
+    for (int s : prefill_seqs) {
+      const int n = qo_indptr[s + 1] - qo_indptr[s], L = seq_lens[s];
+      for (int t0 = 0; t0 < n; t0 += 2 * tile_tokens)
+        work += (L - n + std::min(n, t0 + 2 * tile_tokens) + block_size - 1) / block_size;
+    }
+    piece_pages = std::max<int64_t>(32, work * num_kv_heads / (static_cast<int64_t>(num_sms) * 3));
+  }
   for (int s : prefill_seqs) {
     const int n = qo_indptr[s + 1] - qo_indptr[s], L = seq_lens[s];
     for (int t0 = 0; t0 < n; t0 += 2 * tile_tokens) {
       const int ntok[2] = {std::min(tile_tokens, n - t0), std::max(0, std::min(tile_tokens, n - t0 - tile_tokens))};
       const int key_end = L - n + t0 + ntok[0] + ntok[1];  // keys 0 .. key_end - 1: the pair's last token
       const int pages = (key_end + block_size - 1) / block_size;
-      int pieces = std::min(255, std::max(1, (pages + kPrefillPiecePages - 1) / kPrefillPiecePages));
+      int pieces = static_cast<int>(std::min<int64_t>(255, std::max<int64_t>(1, (pages + piece_pages - 1) / piece_pages)));
       int per = (pages + pieces - 1) / pieces;
       per = (per + kMinPagesPerUnit - 1) / kMinPagesPerUnit * kMinPagesPerUnit;  // whole 8-page MMA tiles
       pieces = (pages + per - 1) / per;

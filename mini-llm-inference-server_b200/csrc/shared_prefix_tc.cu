@@ -36,12 +36,11 @@
 // TMEM columns, paired: S_A [0,128), S_B [128,256), O_A [256, 256 + Dh), O_B [256 + Dh, 256 + 2 Dh);
 // single: S buffers [0,128), [128,256), [256,384), O [384, 384 + Dh).
 //
-// 4-bit pools (FP4; fp4.cuh) take the same kernel with other feeders: 512 threads, warps 12-15 load each tile's codes
-// (thread = key row, one tile ahead, in registers), widen them to fp16 (code * scale, exact) and store them where
-// TMA would have put them; rows that must not be seen (a bad block id, past the sequence's end) are stored as
-// zeros, so nothing is cleared later.  About 160 instructions a thread and tile of 128 x 128, a fifth of a tile's
-// time beside the softmax.  Q and P are fp16 for both output types: a bf16 query row is divided by the power of
-// two of its largest element (exact), which goes into the row's softmax scale.
+// 4-bit pools (FP4; fp4.cuh) take the same kernel with other feeders: warps 0, 2 and 3 (for a single tile K only, and
+// the idle softmax warpgroup V) load key rows' codes into registers, two steps ahead, widen them to fp16 (code * scale,
+// exact) and store them where TMA would have put them; rows that must not be seen (a bad block id, past the sequence's
+// end) are stored as zeros, so nothing is cleared later.  Q and P are fp16 for both output types: a bf16 query row is
+// divided by the power of two of its largest element (exact), which goes into the row's softmax scale.
 //
 // Every wait is bounded (time and polls); on expiry the CTA raises MLB_DEV_WAIT_TIMEOUT, drains its own
 // copies and MMAs, frees TMEM and returns.
@@ -61,22 +60,21 @@ namespace mlb {
 
 namespace {
 
-// 12 warps: 3 producers, the MMA issuer, two softmax warpgroups; 4-bit pools: the issuer's warpgroup, two softmax
-// warpgroups and one that widens codes
-template <bool FP4>
-constexpr int kTcThreads = FP4 ? 512 : 384;
+constexpr int kTcThreads = 384;     // 12 warps: 3 producers, the MMA issuer, two softmax warpgroups
 constexpr int kTcRows = 128;        // query columns per tile = MMA M = TMEM lanes
 constexpr int kTcTileTokens = 128;  // keys per tile = N of S = Q . K^T
 constexpr int kTcTilePages = kTcTileTokens / kBlockSize;
 constexpr uint32_t kTmemCols = 512;
-// registers per thread: at launch (384 or 512 threads on one SM), after the split for warps 0-3, for the softmax and
-// for the warps that widen codes
+// registers per thread: at launch (384 threads on one SM), after the split for warps 0-3 and for the softmax (4-bit
+// feeders hold two rows of codes)
+constexpr int kRegsLaunch = 168;
 template <bool FP4>
-struct TcRegs {
-  static constexpr int kLaunch = FP4 ? 128 : 168, kLow = FP4 ? 40 : 56, kHigh = FP4 ? 208 : 224, kFeed = FP4 ? 56 : 0;
-  static_assert(128 * kLow + 256 * kHigh + 128 * kFeed == kLaunch * kTcThreads<FP4>, "the split must balance");
-  static_assert(kLaunch * kTcThreads<FP4> <= 65536, "one CTA per SM");
-};
+constexpr int kRegsLow = FP4 ? 72 : 56;
+template <bool FP4>
+constexpr int kRegsHigh = FP4 ? 216 : 224;
+static_assert(128 * (kRegsLaunch - kRegsLow<true>) == 256 * (kRegsHigh<true> - kRegsLaunch), "the split must balance");
+static_assert(128 * (kRegsLaunch - kRegsLow<false>) == 256 * (kRegsHigh<false> - kRegsLaunch), "the split must balance");
+static_assert(kRegsLaunch * kTcThreads <= 65536, "one CTA per SM");
 // TMEM columns: S_A [0,128), S_B [128,256), O_A [256, 256 + Dh), O_B after it; P_x (16-bit pairs) over the
 // first 64 columns of S_x
 __device__ __forceinline__ uint32_t col_s(int x) { return x ? 128u : 0u; }
@@ -114,10 +112,11 @@ __device__ __forceinline__ uint32_t sw_chunk(int r, int c) {
 template <int DH>
 struct FeedRow {
   uint32_t w[DH / 8];
-  uint32_t scales[DH / 128 > 0 ? DH / 128 : 1];  // a byte for each run of 32 dims
-  __device__ __forceinline__ void load(const uint8_t* rec, int t) {  // rec == nullptr: a key that reads as zeros
+  uint32_t scales;  // a byte for each run of 32 dims (Dh <= 128)
+  __device__ __forceinline__ void load(const uint8_t* pool, int64_t off, int t) {  // off < 0: zeros
     constexpr int RUNS = DH / kFp4Run;
-    if (rec) {
+    if (off >= 0) {
+      const uint8_t* rec = pool + off;
       const uint4* src = reinterpret_cast<const uint4*>(rec + t * Fp4<DH>::kRow);
 #pragma unroll
       for (int i = 0; i < DH / 32; ++i) {
@@ -128,18 +127,18 @@ struct FeedRow {
 #pragma unroll
       for (int r = 0; r < RUNS; ++r)
         b |= static_cast<uint32_t>(__ldg(rec + Fp4<DH>::kScales + fp4_scale_at(r, t))) << (8 * r);
-      scales[0] = b;
+      scales = b;
     } else {
 #pragma unroll
       for (int i = 0; i < DH / 8; ++i) w[i] = 0u;
-      scales[0] = 0u;
+      scales = 0u;
     }
   }
   // row `row` of a [DH/64][128][64] swizzled fp16 tile
   __device__ __forceinline__ void store(uint32_t tile, int row) const {
 #pragma unroll
     for (int c = 0; c < DH / 8; ++c) {
-      const uint32_t s = ((scales[0] >> (8 * (c / 4))) & 0xffu) * 0x00010001u << 7;
+      const uint32_t s = ((scales >> (8 * (c / 4))) & 0xffu) * 0x00010001u << 7;
       uint32_t x[4];
       fp4_unpack8(w[c], x[0], x[1], x[2], x[3]);
 #pragma unroll
@@ -151,8 +150,94 @@ struct FeedRow {
   }
 };
 
+// Where the key rows of a CTA's tiles lie in a 4-bit pool.
+template <int DH>
+struct TileRows {
+  const int32_t* ids;  // block ids of the unit's pages
+  int64_t block_bytes, head_off, num_blocks;
+  int len, npages;  // keys of the sequence from the unit's first page on; pages of the unit
+  int32_t* err;
+  __device__ __forceinline__ TileRows(const AttnArgs& a, int kvh, int seq_len, const int32_t* table, int begin, int pages)
+      : ids(table), block_bytes(static_cast<int64_t>(a.hkv) * Fp4<DH>::kRecord),
+        head_off(static_cast<int64_t>(kvh) * Fp4<DH>::kRecord), num_blocks(a.num_blocks),
+        len(seq_len == INT_MAX ? INT_MAX : seq_len - begin * kBlockSize), npages(pages), err(a.err) {}
+  // block id of key `key`'s page (counted from the unit's first); INT_MIN: a key that reads as zeros
+  __device__ __forceinline__ int id(int key) const {
+    const int page = key / kBlockSize;
+    return page < npages && key < len ? __ldg(ids + page) : INT_MIN;
+  }
+  // offset of its record; -1: zeros
+  __device__ __forceinline__ int64_t offset(int bid) const {
+    if (bid >= 0 && bid < num_blocks) return bid * block_bytes + head_off;
+    if (bid != INT_MIN) flag_error(err, MLB_DEV_BLOCK_RANGE);
+    return -1;
+  }
+};
+
+// A warpgroup's threads fill one pool's ring of S stages, thread = key row of every tile, loads issued two tiles
+// ahead (a tile is consumed in ~1.6 us; one tile ahead left ~1 us of every load exposed).
+template <int DH, int S>
+__device__ __forceinline__ void feed_ring(const TileRows<DH>& rows, const uint8_t* pool, int row, uint32_t ring, int ntiles,
+                                          uint64_t* full, uint64_t* empty, volatile int* abort_flag, int32_t* err) {
+  constexpr int kTile = TcLayout<DH>::kTileBytes;
+  FeedRow<DH> r[2];
+  const int t = row % kBlockSize;
+  r[0].load(pool, rows.offset(rows.id(row)), t);
+  r[1].load(pool, rows.offset(rows.id(kTcTileTokens + row)), t);
+  int next = rows.id(2 * kTcTileTokens + row);
+  for (int j0 = 0; j0 < ntiles; j0 += 2) {
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int j = j0 + b;
+      if (j >= ntiles) return;
+      if (j >= S && !tc_wait(empty + j % S, ((j / S) + 1) & 1, abort_flag, err)) return;
+      r[b].store(ring + (j % S) * kTile, row);
+      fence_proxy_async_smem();  // generic-proxy stores, read by the tensor core (async proxy)
+      mbar_arrive(full + j % S);
+      r[b].load(pool, rows.offset(next), t);
+      next = rows.id((j + 3) * kTcTileTokens + row);
+    }
+  }
+}
+
+// Three warps fill the rings of K and V (BOTH) or K alone: a tile is 4 groups of 32 key rows, group n of the whole
+// sequence (K of tile 0, V of tile 0, K of tile 1, ...) goes to warp n % 3, loads issued two of a warp's groups ahead.
+template <int DH, bool BOTH>
+__device__ __forceinline__ void feed_groups(const TileRows<DH>& rows, const AttnArgs& a, int part, int lane, uint32_t k_ring,
+                                            uint32_t v_ring, int ntiles, uint64_t* kfull, uint64_t* kempty, uint64_t* vfull,
+                                            uint64_t* vempty, volatile int* abort_flag) {
+  using L = TcLayout<DH>;
+  constexpr int PER = BOTH ? 8 : 4;  // groups a tile
+  const int total = ntiles * PER, t = lane % kBlockSize;
+  auto key = [&](int n) { return (n / PER) * kTcTileTokens + (n % 4) * 32 + lane; };
+  auto load = [&](FeedRow<DH>& r, int n, int bid) {
+    const bool is_v = BOTH && (n & 4);
+    r.load(reinterpret_cast<const uint8_t*>(is_v ? a.v_cache : a.k_cache), rows.offset(bid), t);
+  };
+  FeedRow<DH> r[2];
+  load(r[0], part, rows.id(key(part)));
+  load(r[1], part + 3, rows.id(key(part + 3)));
+  int next = rows.id(key(part + 6));
+  for (int n0 = part; n0 < total; n0 += 6) {
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int n = n0 + 3 * b;
+      if (n >= total) return;
+      const int j = n / PER, row = (n % 4) * 32 + lane;
+      const bool is_v = BOTH && (n & 4);
+      const int stages = is_v ? L::kVStages : L::kKStages, st = j % stages;
+      if (j >= stages && !tc_wait((is_v ? vempty : kempty) + st, ((j / stages) + 1) & 1, abort_flag, a.err)) return;
+      r[b].store((is_v ? v_ring : k_ring) + st * L::kTileBytes, row);
+      fence_proxy_async_smem();  // generic-proxy stores, read by the tensor core (async proxy)
+      mbar_arrive((is_v ? vfull : kfull) + st);
+      load(r[b], n + 6, next);
+      next = rows.id(key(n + 9));
+    }
+  }
+}
+
 template <int DT, int DH, bool FP4>
-__global__ void __launch_bounds__(kTcThreads<FP4>, 1)
+__global__ void __launch_bounds__(kTcThreads, 1)
     shared_prefix_tc_kernel(AttnArgs a, const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv) {
   using L = TcLayout<DH>;
   constexpr int NK = L::kKStages, NV = L::kVStages;
@@ -229,19 +314,26 @@ __global__ void __launch_bounds__(kTcThreads<FP4>, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  // Register split: the producer / MMA warpgroup (warps 0-3) drops to kLow (and the 4-bit feeders to kFeed), the two
-  // softmax warpgroups take what they free (kHigh each).  The launch gives every thread kLaunch (checked on the host
-  // against the compiled kernel before any launch), so the shares add up to the launch's exactly.
+  // Register split: the producer / MMA warpgroup (warps 0-3) drops to kRegsLow, the two softmax warpgroups
+  // take what it frees (kRegsHigh each).  The launch gives every thread kRegsLaunch (checked on the host
+  // against the compiled kernel before any launch), so 128 x (launch - low) = 256 x (high - launch) exactly.
   if (warp < 4) {
     // warpgroup 0 gives up registers, all four warps at the same instruction
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TcRegs<FP4>::kLow));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLow<FP4>));
     if (warp != 1) {
       // ------------------------------------------------------------ producers: warp 0 fills the K ring,
       // warp 2 the V ring (warp 3 has no role), so a K tile never queues behind a V slot: the K ring runs up
       // to kKStages tiles ahead of the scores while V stages wait for their P . V products.  Lane p loads
       // page p's block id one tile ahead (the table round trip overlaps the previous tile) and issues the
       // page's Dh/64 boxes; lane 0 declares the tile's bytes on the stage barrier (one arrival per phase).
-      if (!FP4 && warp != 3) {
+      if constexpr (FP4) {
+        const TileRows<DH> rows(a, kvh, tile_unit ? __ldg(a.seq_lens + tseq) : INT_MAX, table + pb, pb, npages);
+        const int part = warp ? warp - 1 : 0;  // warps 0, 2, 3
+        if (two)
+          feed_groups<DH, true>(rows, a, part, lane, k_smem, v_smem, ntiles, kfull, kempty, vfull, vempty, abort_flag);
+        else
+          feed_groups<DH, false>(rows, a, part, lane, k_smem, v_smem, ntiles, kfull, kempty, vfull, vempty, abort_flag);
+      } else if (warp != 3) {
         constexpr uint32_t kBoxBytes = 64 * 2 * kBlockSize;  // {64 dims, 1 head, 16 slots}
         constexpr int kHalves = DH / 64;
         const bool is_v = warp == 2;
@@ -386,48 +478,8 @@ __global__ void __launch_bounds__(kTcThreads<FP4>, 1)
         if (!tc_drain(final_bar, 0)) flag_error(a.err, MLB_DEV_WAIT_TIMEOUT);
       }
     }
-  } else if (FP4 && warp >= 12) {
-    if constexpr (FP4) {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TcRegs<FP4>::kFeed));
-      // ---------------------------------------------------------- feeders: thread = key row of every tile.  A row's
-      // loads are issued a tile ahead of its stores, K's while V is stored and the other way round.
-      const int row = threadIdx.x - 384, page_in = row / kBlockSize, t = row % kBlockSize;
-      const int64_t block_bytes = static_cast<int64_t>(a.hkv) * Fp4<DH>::kRecord;
-      const int64_t head_off = static_cast<int64_t>(kvh) * Fp4<DH>::kRecord;
-      const int seq_len = tile_unit ? __ldg(a.seq_lens + tseq) : INT_MAX;
-      auto offset = [&](int j) -> int64_t {  // of the row's page in a pool; -1: nothing to see
-        const int page = j * kTcTilePages + page_in;
-        if (j >= ntiles || page >= npages) return -1;
-        const int bid = __ldg(table + pb + page);
-        if (bid < 0 || bid >= a.num_blocks) {
-          if (t == 0) flag_error(a.err, MLB_DEV_BLOCK_RANGE);
-          return -1;
-        }
-        if ((pb + page) * kBlockSize + t >= seq_len) return -1;
-        return bid * block_bytes + head_off;
-      };
-      const uint8_t* kp = reinterpret_cast<const uint8_t*>(a.k_cache);
-      const uint8_t* vp = reinterpret_cast<const uint8_t*>(a.v_cache);
-      FeedRow<DH> k, v;
-      int64_t off = offset(0);
-      k.load(off < 0 ? nullptr : kp + off, t);
-      v.load(off < 0 ? nullptr : vp + off, t);
-      for (int j = 0; j < ntiles; ++j) {
-        const int64_t next = offset(j + 1);
-        if (j >= NK && !tc_wait(kempty + j % NK, ((j / NK) + 1) & 1, abort_flag, a.err)) break;
-        k.store(k_smem + (j % NK) * L::kTileBytes, row);
-        fence_proxy_async_smem();  // generic-proxy stores, read by the tensor core (async proxy)
-        mbar_arrive(kfull + j % NK);
-        k.load(next < 0 ? nullptr : kp + next, t);
-        if (j >= NV && !tc_wait(vempty + j % NV, ((j / NV) + 1) & 1, abort_flag, a.err)) break;
-        v.store(v_smem + (j % NV) * L::kTileBytes, row);
-        fence_proxy_async_smem();
-        mbar_arrive(vfull + j % NV);
-        v.load(next < 0 ? nullptr : vp + next, t);
-      }
-    }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TcRegs<FP4>::kHigh));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsHigh<FP4>));
     // ------------------------------------------------------------ softmax warpgroups: warps 4-7 take tile A,
     // warps 8-11 tile B; one thread = one query column = one TMEM lane
     const int x = warp >= 8 ? 1 : 0;
@@ -482,6 +534,12 @@ __global__ void __launch_bounds__(kTcThreads<FP4>, 1)
     }
     mbar_arrive(q_ready);
     const bool active = x == 0 || two;
+    if constexpr (FP4) {
+      if (!active)  // a single tile leaves this warpgroup without scores: it feeds V
+        feed_ring<DH, NV>(TileRows<DH>(a, kvh, tile_unit ? __ldg(a.seq_lens + tseq) : INT_MAX, table + pb, pb, npages),
+                          reinterpret_cast<const uint8_t*>(a.v_cache), row, v_smem, ntiles, vfull, vempty, abort_flag,
+                          a.err);
+    }
     // this column's destination: an unsplit query tile writes its final row, everything else a split-K
     // partial row (its index read now, off the epilogue's path)
     const int out_m = row / a.group, out_head = kvh * a.group + row % a.group;
@@ -729,11 +787,11 @@ cudaError_t launch_tc(const AttnArgs& a, int64_t units, cudaStream_t s) {
   if (e != cudaSuccess) return e;
   if (!(dev < 64 && (done >> dev) & 1ull)) {
     // the register split inside the kernel (setmaxnreg) balances only if every thread starts with exactly
-    // kLaunch registers; a build that compiled to another count is refused instead of launched
+    // kRegsLaunch registers; a build that compiled to another count is refused instead of launched
     cudaFuncAttributes fa{};
     e = cudaFuncGetAttributes(&fa, k);
     if (e != cudaSuccess) return e;
-    if (fa.numRegs != TcRegs<FP4>::kLaunch) return cudaErrorInvalidKernelImage;
+    if (fa.numRegs != kRegsLaunch) return cudaErrorInvalidKernelImage;
     e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return e;
     if (dev < 64) __atomic_fetch_or(&done, 1ull << dev, __ATOMIC_RELAXED);
@@ -745,7 +803,7 @@ cudaError_t launch_tc(const AttnArgs& a, int64_t units, cudaStream_t s) {
     if (e != cudaSuccess) return e;
   }
   // one CTA per pair of units (2i, 2i + 1) and KV head
-  return launch_k(k, dim3(static_cast<unsigned>(units / 2 * a.hkv)), dim3(kTcThreads<FP4>), bytes, s, a, tk, tv);
+  return launch_k(k, dim3(static_cast<unsigned>(units / 2 * a.hkv)), dim3(kTcThreads), bytes, s, a, tk, tv);
 }
 
 }  // namespace

@@ -8,7 +8,6 @@ error word instead of faulting the GPU.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import math
 from dataclasses import dataclass
@@ -308,10 +307,9 @@ def can_fuse_append(plan: AttentionPlan, k_cache: torch.Tensor, k: torch.Tensor,
 
 def splitk_reduce(plan: AttentionPlan, workspace: Workspace, out: torch.Tensor | None,
                   targets: OutTargets | None = None, dtype: torch.dtype | None = None, head_dim: int | None = None,
-                  device: torch.device | None = None, wide: bool = False) -> None:
+                  device: torch.device | None = None) -> None:
     """K2b: combine the split sequences' partial rows into `out` (no-op when the plan split nothing).
-    With `targets`, the rows go there instead; dtype / head_dim / device then describe them.  `wide` shares a
-    token's pieces between the warps of a CTA (few tokens of many pieces)."""
+    With `targets`, the rows go there instead; dtype / head_dim / device then describe them."""
     if not plan.num_partial_rows or plan.num_tokens == 0:
         return
     if targets is None:
@@ -320,10 +318,9 @@ def splitk_reduce(plan: AttentionPlan, workspace: Workspace, out: torch.Tensor |
         dtype, head_dim, device = out.dtype, out.shape[2], out.device
     n, h = plan.num_tokens, plan.num_heads
     po, plse = workspace.get(plan.num_partial_rows, h, head_dim, device)
-    reduce = lib().mlb_splitk_reduce_wide if wide else lib().mlb_splitk_reduce
-    rc = reduce(po.data_ptr(), plse.data_ptr(), plan.num_partial_rows, plan.reduce_rows.data_ptr(),
-                plan.reduce_chunks.data_ptr(), plan.tokens_per_tile, n, h, head_dim, _ptr(out), *_strides(out),
-                DTYPE_CODE[dtype], _targets(targets), _stream(device))
+    rc = lib().mlb_splitk_reduce(po.data_ptr(), plse.data_ptr(), plan.num_partial_rows, plan.reduce_rows.data_ptr(),
+                                 plan.reduce_chunks.data_ptr(), plan.tokens_per_tile, n, h, head_dim, _ptr(out),
+                                 *_strides(out), DTYPE_CODE[dtype], _targets(targets), _stream(device))
     check(rc, "splitk_reduce")
 
 
@@ -392,15 +389,33 @@ def fp4_pool_shape(num_blocks: int, num_kv_heads: int, head_dim: int) -> tuple[i
     return num_blocks, num_kv_heads, FP4_ROWS, head_dim // 2
 
 
-def _on(device: torch.device):
-    """The launches' device made current, if it is not already."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def _launch(fn, what: str, device: int, *args) -> None:
+    """Call an entry point with the current stream of `device` (an ordinal), made current if it is not already."""
+    if _current_device() == device:
+        rc = fn(*args, _raw_stream(device) if _raw_stream else torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    if rc:
+        check(rc, what)
+
+
+# A decode step makes several of these calls per layer, each a few microseconds on the GPU: every entry point below
+# tests its arguments with one expression of cheap attributes, and only where that fails with the checks that say what
+# is wrong (or that the case is an uncommon one that is fine: an empty tensor's strides).
 
 
 def _check_fp4_pools(k_cache: torch.Tensor, v_cache: torch.Tensor, what: str) -> tuple[int, int, int]:
     """(num_blocks, Hkv, Dh) of a pair of 4-bit pools."""
+    shape = k_cache.shape
+    dev = k_cache.get_device()
+    if (len(shape) == 4 and shape[2] == FP4_ROWS and dev >= 0 and k_cache.dtype is torch.uint8
+            and k_cache.is_contiguous() and v_cache.shape == shape and v_cache.dtype is torch.uint8
+            and v_cache.is_contiguous() and v_cache.get_device() == dev):
+        return shape[0], shape[1], 2 * shape[3]
     _check_pool(k_cache, what)
     _check_pool(v_cache, what)
     if k_cache.dtype is not torch.uint8 or k_cache.shape[2] != FP4_ROWS:
@@ -411,10 +426,10 @@ def _check_fp4_pools(k_cache: torch.Tensor, v_cache: torch.Tensor, what: str) ->
     return k_cache.shape[0], k_cache.shape[1], 2 * k_cache.shape[3]
 
 
-def _check_index(t: torch.Tensor, n: int, device: torch.device, what: str) -> None:
+def _check_index(t: torch.Tensor, n: int, device: torch.device, what: str, name: str) -> None:
     if t.dtype is not torch.long or t.shape != (n,) or not t.is_contiguous() or t.device != device:
-        raise ValueError(f"{what} must be a contiguous int64 [{n}] tensor on {device}, got {t.dtype} {tuple(t.shape)} "
-                         f"on {t.device}")
+        raise ValueError(f"{what}: {name} must be a contiguous int64 [{n}] tensor on {device}, got {t.dtype} "
+                         f"{tuple(t.shape)} on {t.device}")
 
 
 def kv_append_fp4(k_cache: torch.Tensor, v_cache: torch.Tensor, slot_mapping: torch.Tensor, k: torch.Tensor,
@@ -422,44 +437,45 @@ def kv_append_fp4(k_cache: torch.Tensor, v_cache: torch.Tensor, slot_mapping: to
     """`kv_append` into 4-bit pools: rows k[i] / v[i] (float32, float16 or bfloat16, strided views allowed) are
     rounded to e2m1 codes with a scale for each 32 dims (mlb_kv_append_fp4) and stored at slot_mapping[i].  Slots
     must be distinct."""
-    nb, hkv, dh = _check_fp4_pools(k_cache, v_cache, "kv_append_fp4")
-    _check_rows(k, hkv, dh, "kv_append_fp4 k")
-    _check_rows(v, hkv, dh, "kv_append_fp4 v")
-    n = k.shape[0]
-    if v.shape[0] != n or k.dtype != v.dtype:
-        raise ValueError(f"kv_append_fp4: k and v differ ({tuple(k.shape)} {k.dtype}, {tuple(v.shape)} {v.dtype})")
-    if k.device != k_cache.device or v.device != k_cache.device:
-        raise ValueError("kv_append_fp4: all tensors must be on the pools' device")
-    _check_index(slot_mapping, n, k_cache.device, "kv_append_fp4: slot_mapping")
-    code = _code(k, "kv_append_fp4")
-    if n == 0:
-        return
-    with _on(k_cache.device):
-        rc = lib().mlb_kv_append_fp4(k_cache.data_ptr(), v_cache.data_ptr(), nb, slot_mapping.data_ptr(), k.data_ptr(),
-                                     k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), code, n, hkv,
-                                     dh, _ptr(err), _stream(k_cache.device))
-    check(rc, "kv_append_fp4")
+    what = "kv_append_fp4"
+    nb, hkv, dh = _check_fp4_pools(k_cache, v_cache, what)
+    dev, shape, ks, vs, code = k_cache.get_device(), k.shape, k.stride(), v.stride(), DTYPE_CODE.get(k.dtype)
+    if not (len(shape) == 3 and shape[1] == hkv and shape[2] == dh and v.shape == shape and ks[2] == 1 and vs[2] == 1
+            and code is not None and v.dtype is k.dtype and k.get_device() == dev and v.get_device() == dev
+            and slot_mapping.dtype is torch.long and slot_mapping.shape == shape[:1] and slot_mapping.is_contiguous()
+            and slot_mapping.get_device() == dev):
+        _check_rows(k, hkv, dh, f"{what} k")
+        _check_rows(v, hkv, dh, f"{what} v")
+        if v.shape[0] != shape[0] or k.dtype != v.dtype:
+            raise ValueError(f"{what}: k and v differ ({tuple(k.shape)} {k.dtype}, {tuple(v.shape)} {v.dtype})")
+        if k.device != k_cache.device or v.device != k_cache.device:
+            raise ValueError(f"{what}: all tensors must be on the pools' device")
+        _check_index(slot_mapping, shape[0], k_cache.device, what, "slot_mapping")
+        _code(k, what)
+    if shape[0]:
+        _launch(lib().mlb_kv_append_fp4, what, dev, k_cache.data_ptr(), v_cache.data_ptr(), nb, slot_mapping.data_ptr(),
+                k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], code, shape[0], hkv, dh, _ptr(err))
 
 
 def kv_read_fp4(k_cache: torch.Tensor, v_cache: torch.Tensor, slot_mapping: torch.Tensor,
                 dtype: torch.dtype = torch.bfloat16, err: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """The values that 4-bit pools hold at slot_mapping: (k, v) rows [N, Hkv, Dh] of `dtype` (exact in all three).
     The same slot may be asked for more than once; a slot out of range reads as zeros."""
-    nb, hkv, dh = _check_fp4_pools(k_cache, v_cache, "kv_read_fp4")
+    what = "kv_read_fp4"
+    nb, hkv, dh = _check_fp4_pools(k_cache, v_cache, what)
     if dtype not in DTYPE_CODE:
-        raise ValueError(f"kv_read_fp4: dtype {dtype} not supported (float32, float16, bfloat16)")
+        raise ValueError(f"{what}: dtype {dtype} not supported (float32, float16, bfloat16)")
     if slot_mapping.dim() != 1:
-        raise ValueError("kv_read_fp4: slot_mapping must be 1-D")
+        raise ValueError(f"{what}: slot_mapping must be 1-D")
     n = slot_mapping.shape[0]
-    _check_index(slot_mapping, n, k_cache.device, "kv_read_fp4: slot_mapping")
-    k = torch.empty((n, hkv, dh), dtype=dtype, device=k_cache.device)
+    dev = k_cache.get_device()
+    if not (slot_mapping.dtype is torch.long and slot_mapping.is_contiguous() and slot_mapping.get_device() == dev):
+        _check_index(slot_mapping, n, k_cache.device, what, "slot_mapping")
+    k = k_cache.new_empty((n, hkv, dh), dtype=dtype)
     v = torch.empty_like(k)
     if n:
-        with _on(k_cache.device):
-            rc = lib().mlb_kv_read_fp4(k_cache.data_ptr(), v_cache.data_ptr(), nb, slot_mapping.data_ptr(),
-                                       k.data_ptr(), v.data_ptr(), DTYPE_CODE[dtype], n, hkv, dh, _ptr(err),
-                                       _stream(k_cache.device))
-        check(rc, "kv_read_fp4")
+        _launch(lib().mlb_kv_read_fp4, what, dev, k_cache.data_ptr(), v_cache.data_ptr(), nb, slot_mapping.data_ptr(),
+                k.data_ptr(), v.data_ptr(), DTYPE_CODE[dtype], n, hkv, dh, _ptr(err))
     return k, v
 
 
@@ -471,39 +487,41 @@ def attention_partials_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     partial rows in `workspace` for `splitk_reduce`."""
     what = "paged_attention_fp4"
     nb, hkv, dh = _check_fp4_pools(k_cache, v_cache, what)
-    if q.dim() != 3 or q.shape[2] != dh or (q.shape[0] and q.stride(2) != 1):
-        raise ValueError(f"{what}: q must be [N, H, {dh}] with unit last stride, got {tuple(q.shape)}")
-    if q.dtype is not torch.bfloat16 and q.dtype is not torch.float16:
-        raise ValueError(f"{what}: q must be float16 or bfloat16, got {q.dtype}")
-    n, h = q.shape[0], q.shape[1]
-    if (plan.num_heads, plan.num_kv_heads, plan.num_tokens) != (h, hkv, n):
-        raise ValueError(f"{what}: the plan was built for another shape")
-    if q.device != k_cache.device:
-        raise ValueError(f"{what}: q must be on the pools' device")
+    dev, shape, qs, code = q.get_device(), q.shape, q.stride(), DTYPE_CODE.get(q.dtype)
+    if not (len(shape) == 3 and shape[2] == dh and qs[2] == 1 and (code == _lib.MLB_F16 or code == _lib.MLB_BF16)
+            and dev == k_cache.get_device() and plan.num_tokens == shape[0] and plan.num_heads == shape[1]
+            and plan.num_kv_heads == hkv):
+        if len(shape) != 3 or shape[2] != dh or (shape[0] and qs[2] != 1):
+            raise ValueError(f"{what}: q must be [N, H, {dh}] with unit last stride, got {tuple(q.shape)}")
+        if q.dtype is not torch.bfloat16 and q.dtype is not torch.float16:
+            raise ValueError(f"{what}: q must be float16 or bfloat16, got {q.dtype}")
+        if (plan.num_heads, plan.num_kv_heads, plan.num_tokens) != (shape[1], hkv, shape[0]):
+            raise ValueError(f"{what}: the plan was built for another shape")
+        if q.device != k_cache.device:
+            raise ValueError(f"{what}: q must be on the pools' device")
     for t, name in ((block_tables, "block_tables"), (seq_lens, "seq_lens"), (qo_indptr, "qo_indptr"),
                     (plan.units, "the plan")):
-        if t.dtype is not torch.int32 or not t.is_contiguous() or t.device != q.device:
+        if t.dtype is not torch.int32 or not t.is_contiguous() or t.get_device() != dev:
             raise ValueError(f"{what}: {name} must be a contiguous int32 tensor on {q.device}")
+    n, h, _ = shape
     if targets is not None:
-        out = None
-    elif out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or (n and out.stride(2) != 1):
-        raise ValueError(f"{what}: out must match q")
+        out, o0, o1 = None, 0, 0
+    else:
+        if out is None:
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        elif out.shape != shape or out.dtype != q.dtype or out.get_device() != dev or (n and out.stride(2) != 1):
+            raise ValueError(f"{what}: out must match q")
+        o0, o1, _ = out.stride()
     if n == 0 or plan.num_units + plan.num_shared_units == 0:
         return out
-    scale = 1.0 / math.sqrt(dh) if scale is None else float(scale)
     po = plse = None
     if plan.num_partial_rows:
         po, plse = workspace.get(plan.num_partial_rows, h, dh, q.device)
-    with _on(q.device):
-        rc = lib().mlb_paged_attention_fp4(
-            q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), DTYPE_CODE[q.dtype], nb, h,
-            hkv, dh, scale, block_tables.data_ptr(), block_tables.stride(0), seq_lens.data_ptr(), qo_indptr.data_ptr(),
-            seq_lens.shape[0], plan.units.data_ptr(), plan.num_units, plan.shared_units.data_ptr(),
-            plan.num_shared_units, plan.members.data_ptr(), _ptr(po), _ptr(plse), plan.num_partial_rows, _ptr(out),
-            *_strides(out), _targets(targets), _ptr(err), _stream(q.device))
-    check(rc, what)
+    _launch(lib().mlb_paged_attention_fp4, what, dev, q.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(),
+            code, nb, h, hkv, dh, 1.0 / math.sqrt(dh) if scale is None else float(scale), block_tables.data_ptr(),
+            block_tables.stride(0), seq_lens.data_ptr(), qo_indptr.data_ptr(), seq_lens.shape[0], plan.units.data_ptr(),
+            plan.num_units, plan.shared_units.data_ptr(), plan.num_shared_units, plan.members.data_ptr(), _ptr(po),
+            _ptr(plse), plan.num_partial_rows, _ptr(out), o0, o1, _targets(targets), _ptr(err))
     return out
 
 
@@ -517,9 +535,14 @@ def paged_attention_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     workspace = workspace or Workspace()
     out = attention_partials_fp4(q, k_cache, v_cache, block_tables, seq_lens, qo_indptr, plan, workspace, out, scale,
                                  err, targets)
-    with _on(q.device):
-        splitk_reduce(plan, workspace, out, targets, q.dtype, q.shape[2], q.device,
-                      wide=plan.max_pieces > WIDE_REDUCE_PIECES)
+    if plan.num_partial_rows and plan.num_tokens:
+        dev = q.get_device()
+        po, plse = workspace.get(plan.num_partial_rows, plan.num_heads, q.shape[2], q.device)
+        wide = plan.max_pieces > WIDE_REDUCE_PIECES
+        _launch(lib().mlb_splitk_reduce_wide if wide else lib().mlb_splitk_reduce, "splitk_reduce", dev, po.data_ptr(),
+                plse.data_ptr(), plan.num_partial_rows, plan.reduce_rows.data_ptr(), plan.reduce_chunks.data_ptr(),
+                plan.tokens_per_tile, plan.num_tokens, plan.num_heads, q.shape[2], _ptr(out), *_strides(out),
+                DTYPE_CODE[q.dtype], _targets(targets))
     return out
 
 
@@ -556,6 +579,18 @@ class Rotary:
 
 def _check_rope(what: str, q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor,
                 q_weight: torch.Tensor | None, k_weight: torch.Tensor | None) -> int:
+    qs, dt, dev, code = q.shape, q.dtype, q.get_device(), DTYPE_CODE.get(q.dtype)
+    ks = k.shape
+    if (len(qs) == 3 and len(ks) == 3 and qs[0] == ks[0] and qs[2] == ks[2] and qs[2] in (64, 128, 256)
+            and q.stride()[2] == 1 and k.stride()[2] == 1 and code is not None and k.dtype is dt and dev >= 0
+            and k.get_device() == dev and positions.dtype is torch.long and positions.shape == qs[:1]
+            and positions.is_contiguous() and positions.get_device() == dev and cos_sin.dtype is torch.float32
+            and cos_sin.dim() == 2 and cos_sin.is_contiguous() and cos_sin.get_device() == dev
+            and (q_weight is None or (q_weight.shape == qs[2:] and q_weight.dtype is dt and q_weight.is_contiguous()
+                                      and q_weight.get_device() == dev))
+            and (k_weight is None or (k_weight.shape == qs[2:] and k_weight.dtype is dt and k_weight.is_contiguous()
+                                      and k_weight.get_device() == dev))):
+        return code
     if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
         raise ValueError(f"{what}: q must be [N, H, Dh] and k [N, Hkv, Dh], got {tuple(q.shape)}, {tuple(k.shape)}")
     dh = q.shape[2]
@@ -565,7 +600,7 @@ def _check_rope(what: str, q: torch.Tensor, k: torch.Tensor, positions: torch.Te
         raise ValueError(f"{what}: q and k must be CUDA tensors of one dtype on one device")
     if dh not in (64, 128, 256):
         raise ValueError(f"{what}: head_dim {dh} (supported: 64, 128, 256)")
-    _check_index(positions, q.shape[0], q.device, f"{what}: positions")
+    _check_index(positions, q.shape[0], q.device, what, "positions")
     if (cos_sin.dtype is not torch.float32 or cos_sin.dim() != 2 or not cos_sin.is_contiguous()
             or cos_sin.device != q.device):
         raise ValueError(f"{what}: cos_sin must be a contiguous float32 [num_positions, rot_dim] tensor on {q.device}")
@@ -599,20 +634,19 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, cos_
     (q, k)."""
     what = "qk_norm_rope"
     code = _check_rope(what, q, k, positions, cos_sin, q_weight, k_weight)
+    n, h, dh = q.shape
     if out is None:
-        qo, ko = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k))
+        qo = torch.empty_like(q, memory_format=torch.contiguous_format)
+        ko = torch.empty_like(k, memory_format=torch.contiguous_format)
     else:
         qo, ko = out
         _check_row_out(what, qo, q)
         _check_row_out(what, ko, k)
-    n, h, dh = q.shape
-    with _on(q.device):
-        rc = lib().mlb_qk_norm_rope(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-                                    code, n, h, k.shape[1], dh, positions.data_ptr(), cos_sin.data_ptr(),
-                                    cos_sin.shape[0], cos_sin.shape[1], _ptr(q_weight), _ptr(k_weight), eps,
-                                    qo.data_ptr(), qo.stride(0), qo.stride(1), ko.data_ptr(), ko.stride(0),
-                                    ko.stride(1), _ptr(err), _stream(q.device))
-    check(rc, what)
+    qs, ks, qos, kos = q.stride(), k.stride(), qo.stride(), ko.stride()
+    rows, rot = cos_sin.shape
+    _launch(lib().mlb_qk_norm_rope, what, q.get_device(), q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], code,
+            n, h, k.shape[1], dh, positions.data_ptr(), cos_sin.data_ptr(), rows, rot, _ptr(q_weight), _ptr(k_weight),
+            eps, qo.data_ptr(), qos[0], qos[1], ko.data_ptr(), kos[0], kos[1], _ptr(err))
     return qo, ko
 
 
@@ -626,23 +660,26 @@ def qk_norm_rope_append_fp4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, p
     what = "qk_norm_rope_append_fp4"
     nb, hkv, dh = _check_fp4_pools(k_cache, v_cache, what)
     code = _check_rope(what, q, k, positions, cos_sin, q_weight, k_weight)
-    n, h = q.shape[:2]
-    _check_rows(k, hkv, dh, f"{what} k")
-    _check_rows(v, hkv, dh, f"{what} v")
-    if v.shape[0] != n or v.dtype != k.dtype or v.device != k.device or k_cache.device != k.device:
-        raise ValueError(f"{what}: q, k, v and the pools must agree in rows, dtype and device")
-    _check_index(slot_mapping, n, q.device, f"{what}: slot_mapping")
+    n, h, _ = q.shape
+    dev, ks, vs = q.get_device(), k.stride(), v.stride()
+    if not (k.shape[1] == hkv and k.shape[2] == dh and v.shape == k.shape and vs[2] == 1 and v.dtype is k.dtype
+            and v.get_device() == dev and k_cache.get_device() == dev and slot_mapping.dtype is torch.long
+            and slot_mapping.shape == q.shape[:1] and slot_mapping.is_contiguous() and slot_mapping.get_device() == dev):
+        _check_rows(k, hkv, dh, f"{what} k")
+        _check_rows(v, hkv, dh, f"{what} v")
+        if v.shape[0] != n or v.dtype != k.dtype or v.device != k.device or k_cache.device != k.device:
+            raise ValueError(f"{what}: q, k, v and the pools must agree in rows, dtype and device")
+        _check_index(slot_mapping, n, q.device, what, "slot_mapping")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         _check_row_out(what, out, q)
-    with _on(q.device):
-        rc = lib().mlb_qk_norm_rope_append_fp4(
-            q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
-            v.stride(1), code, n, h, hkv, dh, positions.data_ptr(), cos_sin.data_ptr(), cos_sin.shape[0],
-            cos_sin.shape[1], _ptr(q_weight), _ptr(k_weight), eps, out.data_ptr(), out.stride(0), out.stride(1),
-            k_cache.data_ptr(), v_cache.data_ptr(), nb, slot_mapping.data_ptr(), _ptr(err), _stream(q.device))
-    check(rc, what)
+    qs, os = q.stride(), out.stride()
+    rows, rot = cos_sin.shape
+    _launch(lib().mlb_qk_norm_rope_append_fp4, what, dev, q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1],
+            v.data_ptr(), vs[0], vs[1], code, n, h, hkv, dh, positions.data_ptr(), cos_sin.data_ptr(), rows, rot,
+            _ptr(q_weight), _ptr(k_weight), eps, out.data_ptr(), os[0], os[1], k_cache.data_ptr(), v_cache.data_ptr(), nb,
+            slot_mapping.data_ptr(), _ptr(err))
     return out
 
 
