@@ -39,8 +39,8 @@ cudaError_t launch_splitk_reduce_exchange(const float* po, const float* plse, co
                                           int world, uint32_t* state, int64_t timeout_ns, int32_t* err, int num_sms,
                                           cudaStream_t s);
 cudaError_t launch_norm_rope(const RowArgs& a, int dtype, int dh, bool append, int num_sms, cudaStream_t s);
-cudaError_t launch_fp4_append(const RowArgs& a, int dtype, int dh, int num_sms, cudaStream_t s);
-cudaError_t launch_fp4_read(const RowArgs& a, int dtype, int dh, int num_sms, cudaStream_t s);
+cudaError_t launch_fp4_append(const RowArgs& a, int dtype, int dh, cudaStream_t s);
+cudaError_t launch_fp4_read(const RowArgs& a, int dtype, int dh, cudaStream_t s);
 cudaError_t launch_fp4_attention(const AttnArgs& a, int dtype, int dh, int64_t num_units, cudaStream_t s);
 cudaError_t launch_fp4_shared(const AttnArgs& a, int dtype, int dh, int64_t num_units, cudaStream_t s);
 bool fp4_shared_tc_supported(const AttnArgs& a, int dh);
@@ -891,7 +891,9 @@ int row_shapes(const char* what, int dtype, int64_t num_tokens, int num_heads, i
   if (num_tokens < 0 || num_heads < 0 || num_kv_heads < 0 || num_heads + num_kv_heads <= 0)
     return fail(MLB_EINVAL, "%s: bad sizes", what);
   if (!fp4_head_dim(head_dim)) return fail(MLB_EUNSUPPORTED, "%s: head_dim %d (supported: 64, 128, 256)", what, head_dim);
-  if (num_tokens > (int64_t(1) << 31) / std::max(1, num_heads + 2 * num_kv_heads))
+  // thread indexes are 32-bit: head_dim / 16 threads a row, a warp at least a token
+  const int64_t threads = (static_cast<int64_t>(num_heads) + 2 * static_cast<int64_t>(num_kv_heads)) * (head_dim / 16) + 32;
+  if (num_tokens > (int64_t(1) << 31) / threads)
     return fail(MLB_EINVAL, "%s: %lld tokens of %d heads are too many rows for one launch", what,
                 static_cast<long long>(num_tokens), num_heads + 2 * num_kv_heads);
   return MLB_OK;
@@ -994,7 +996,7 @@ int mlb_kv_append_fp4(void* k_cache, void* v_cache, int64_t num_blocks, const in
   a.slots = slot_mapping, a.num_slots = num_blocks * mlb::kBlockSize;
   a.vec = rows_aligned(k, k_stride_tok, k_stride_head, eb) && rows_aligned(v, v_stride_tok, v_stride_head, eb);
   a.err = err_word;
-  return cuda_status(mlb::launch_fp4_append(a, in_dtype, head_dim, sm_count(), static_cast<cudaStream_t>(stream)),
+  return cuda_status(mlb::launch_fp4_append(a, in_dtype, head_dim, static_cast<cudaStream_t>(stream)),
                      "kv_append_fp4 launch");
 }
 
@@ -1013,7 +1015,7 @@ int mlb_kv_read_fp4(const void* k_cache, const void* v_cache, int64_t num_blocks
   a.v_cache = static_cast<uint8_t*>(const_cast<void*>(v_cache));
   a.slots = slot_mapping, a.num_slots = num_blocks * mlb::kBlockSize;
   a.err = err_word;
-  return cuda_status(mlb::launch_fp4_read(a, out_dtype, head_dim, sm_count(), static_cast<cudaStream_t>(stream)),
+  return cuda_status(mlb::launch_fp4_read(a, out_dtype, head_dim, static_cast<cudaStream_t>(stream)),
                      "kv_read_fp4 launch");
 }
 

@@ -56,36 +56,49 @@ __device__ __forceinline__ uint32_t fp4_pack8(const float (&r)[8]) {
   return w;
 }
 
-// Scale byte of a run whose largest finite magnitude is amax (clamped to kFp4TopValue by the caller):
-// amax / 6 rounded once to the byte format, ties to even.  The quotient is cut (towards zero) and its last bit set
-// when anything was cut off, so the second rounding sees which side of a tie the true quotient lies on.
-__device__ __forceinline__ uint32_t fp4_scale_byte(float amax) {
-  float y = __fdiv_rz(amax, 6.f);
-  if (fmaf(-y, 6.f, amax) != 0.f) y = __uint_as_float(__float_as_uint(y) | 1u);
-  if (y < 6.103515625e-05f) return static_cast<uint32_t>(rintf(y * 131072.f));  // below 2^-14: steps of 2^-17
+// y = amax / 6 (exact, or cut towards zero with its last bit set) -> the nearest scale byte, ties to even.
+__device__ __forceinline__ uint32_t fp4_round_scale(float y) {
+  if (y < 6.103515625e-05f) return static_cast<uint32_t>(__float2uint_rn(y * 131072.f));  // below 2^-14: steps of 2^-17
   uint32_t u = __float_as_uint(y);
   u += 0x7ffffu + ((u >> 20) & 1u);       // to 3 mantissa bits, nearest even
   return (u >> 20) - ((127u - 15u) << 3);  // exponent bias 15
 }
 
+// Scale byte of a run whose largest magnitude is amax (at most kFp4TopValue).  fp32: the quotient is cut towards zero
+// and its last bit set when anything was cut off, so the rounding to the byte sees which side of a tie the true
+// quotient lies on.
+__device__ __forceinline__ uint32_t fp4_scale_byte(float amax) {
+  float y = __fdiv_rz(amax, 6.f);
+  if (fmaf(-y, 6.f, amax) != 0.f) y = __uint_as_float(__float_as_uint(y) | 1u);
+  return fp4_round_scale(y);
+}
+// The same for an amax of at most 11 significant bits: a product with 1/6 is exact where amax / 6 is a tie (5 bits; all
+// 16 mantissas checked), and elsewhere the quotient lies 2^-11 or more from a tie.
+__device__ __forceinline__ uint32_t fp4_scale_byte_16(float amax) { return fp4_round_scale(amax * (1.f / 6.f)); }
+
 __device__ __forceinline__ float fp4_scale_value(uint32_t byte) {
   return __half2float(__ushort_as_half(static_cast<unsigned short>(byte << 7)));
 }
 
-// x / scale with rounding that never moves a value onto a border between two levels: the Newton step makes exact
-// quotients exact (a border times a scale has 7 significant bits); for fp32 inputs, whose quotients can round onto
-// a border they only lie next to, an inexact quotient is made odd in the direction of its remainder.
-template <bool WIDE>
-__device__ __forceinline__ float fp4_quotient(float x, float scale, float inv) {
-  float q = x * inv;
-  q = fmaf(fmaf(-q, scale, x), inv, q);
-  if constexpr (WIDE) {
-    const float r = fmaf(-q, scale, x);
-    uint32_t u = __float_as_uint(q);
-    if (r != 0.f && !(u & 1u) && (u << 1) != 0u) u += ((__float_as_uint(r) ^ u) >> 31) ? 0xffffffffu : 1u;
-    q = __uint_as_float(u);
-  }
-  return copysignf(q, x);  // the correction would turn -0 into +0
+// 1 / scale as hi + lo, hi at most the true reciprocal (the approximation, within a unit, less one unit) and lo >= 0,
+// together good to 2^-46; zeros for a zero scale.  x * hi + x * lo in one rounding is then exact where x / scale is a
+// border between two levels, keeps the sign of a zero, and for x of at most 11 significant bits crosses no border.
+__device__ __forceinline__ void fp4_reciprocal(float scale, float& hi, float& lo) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(scale));
+  hi = scale > 0.f ? __uint_as_float(__float_as_uint(r) - 1u) : 0.f;
+  lo = scale > 0.f ? fmaf(-hi, scale, 1.f) * hi : 0.f;
+}
+__device__ __forceinline__ float fp4_quotient_16(float x, float hi, float lo) { return fmaf(x, hi, x * lo); }
+
+// The same for fp32 x, whose quotients can round onto a border that they only lie next to: an inexact quotient is made
+// odd in the direction of its remainder.
+__device__ __forceinline__ float fp4_quotient_32(float x, float scale, float hi, float lo) {
+  const float q = fmaf(x, hi, x * lo);
+  const float r = fmaf(-q, scale, x);
+  uint32_t u = __float_as_uint(q);
+  if (r != 0.f && !(u & 1u) && (u << 1) != 0u) u += ((__float_as_uint(r) ^ u) >> 31) ? 0xffffffffu : 1u;
+  return __uint_as_float(u);
 }
 
 // bf16 query rows enter fp16 products divided by the power of two of their largest element mx: down = 2^-e, up = 2^e,

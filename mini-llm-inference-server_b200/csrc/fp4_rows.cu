@@ -19,63 +19,104 @@ namespace mlb {
 
 namespace {
 
-// 8 consecutive elements -> fp32
+// 8 consecutive elements as they lie in memory: four pairs (16-bit types) or eight fp32.  VEC: 16-byte loads and stores
+// (a template parameter: as a branch, the element-wise loads were predicated off and still issued).
 template <int DT>
-__device__ __forceinline__ void load8(const char* p, bool vec, float (&x)[8]) {
-  using T = typename Elt<DT>::T;
-  if (vec) {
-    if constexpr (DT == MLB_F32) {
-      const float4 a = *reinterpret_cast<const float4*>(p), b = *(reinterpret_cast<const float4*>(p) + 1);
-      x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+struct Run8 {
+  static constexpr int kWords = DT == MLB_F32 ? 8 : 4;
+  uint32_t w[kWords];
+
+  template <bool VEC>
+  __device__ __forceinline__ void load(const char* p) {
+    if constexpr (VEC) {
+#pragma unroll
+      for (int i = 0; i < kWords / 4; ++i) {
+        const uint4 x = reinterpret_cast<const uint4*>(p)[i];
+        w[4 * i] = x.x, w[4 * i + 1] = x.y, w[4 * i + 2] = x.z, w[4 * i + 3] = x.w;
+      }
+    } else if constexpr (DT == MLB_F32) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
     } else {
-      const uint4 a = *reinterpret_cast<const uint4*>(p);
-      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+      const uint16_t* e = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = static_cast<uint32_t>(e[2 * i]) | (static_cast<uint32_t>(e[2 * i + 1]) << 16);
+    }
+  }
+  template <bool VEC>
+  __device__ __forceinline__ void store(char* p) const {
+    if constexpr (VEC) {
+#pragma unroll
+      for (int i = 0; i < kWords / 4; ++i)
+        reinterpret_cast<uint4*>(p)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    } else if constexpr (DT == MLB_F32) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) reinterpret_cast<uint32_t*>(p)[i] = w[i];
+    } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if constexpr (DT == MLB_BF16) {
-          x[2 * i] = __uint_as_float(w[i] << 16);
-          x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        } else {
-          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-          x[2 * i] = f.x;
-          x[2 * i + 1] = f.y;
-        }
+        reinterpret_cast<uint16_t*>(p)[2 * i] = static_cast<uint16_t>(w[i]);
+        reinterpret_cast<uint16_t*>(p)[2 * i + 1] = static_cast<uint16_t>(w[i] >> 16);
       }
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = to_f32(reinterpret_cast<const T*>(p)[i]);
   }
-}
-
-template <int DT>
-__device__ __forceinline__ void store8(char* p, bool vec, const float (&x)[8]) {
-  if (vec) {
-    if constexpr (DT == MLB_F32) {
-      reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
-      reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
-    } else {
-      *reinterpret_cast<uint4*>(p) = make_uint4(pack2<DT>(x[0], x[1]), pack2<DT>(x[2], x[3]), pack2<DT>(x[4], x[5]),
-                                                pack2<DT>(x[6], x[7]));
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = 0u;
+  }
+  __device__ __forceinline__ void get(float (&x)[8]) const {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      if constexpr (DT == MLB_F32) {
+        x[i] = __uint_as_float(w[i]);
+      } else if constexpr (DT == MLB_BF16) {
+        x[2 * i] = __uint_as_float(w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+      }
     }
-  } else {
+  }
+  __device__ __forceinline__ void set(const float (&x)[8]) {  // rounds to the type
 #pragma unroll
-    for (int i = 0; i < 8; ++i) store_f32<DT>(p + i * Elt<DT>::bytes, x[i]);
+    for (int i = 0; i < kWords; ++i) {
+      if constexpr (DT == MLB_F32)
+        w[i] = __float_as_uint(x[i]);
+      else
+        w[i] = pack2<DT>(x[2 * i], x[2 * i + 1]);
+    }
+  }
+};
+
+// Where a row of a 4-bit pool lies: its record and its token in the block.
+template <int DH>
+struct SlotRow {
+  uint8_t* rec;
+  int t;
+  __device__ __forceinline__ SlotRow(uint8_t* pool, int64_t slot, int hkv, int head)
+      : rec(pool + (static_cast<uint64_t>(slot) / kBlockSize * hkv + head) * Fp4<DH>::kRecord),
+        t(static_cast<int>(slot) & (kBlockSize - 1)) {}
+};
+
+template <int DH>
+__device__ __forceinline__ void store_codes(const SlotRow<DH>& at, int c, uint32_t wa, uint32_t wb, uint32_t ba, uint32_t bb) {
+  constexpr int HALF = DH / 16;  // chunks of 8 dims in half a head
+  uint32_t* row = reinterpret_cast<uint32_t*>(at.rec + at.t * Fp4<DH>::kRow);
+  row[c] = wa;
+  row[HALF + c] = wb;
+  if ((c & 3) == 0) {
+    at.rec[Fp4<DH>::kScales + fp4_scale_at(c / 4, at.t)] = static_cast<uint8_t>(ba);
+    at.rec[Fp4<DH>::kScales + fp4_scale_at((HALF + c) / 4, at.t)] = static_cast<uint8_t>(bb);
   }
 }
 
-template <int DT>
-__device__ __forceinline__ float round_to(float x) {
-  if constexpr (DT == MLB_F32) return x;
-  if constexpr (DT == MLB_F16) return __half2float(__float2half_rn(x));
-  return __bfloat162float(__float2bfloat16_rn(x));
-}
-
-// Quantise a lane's two runs of 8 dims (chunks ca and cb of 8; the 4 lanes of a run of 32 are neighbours) and
-// store codes and scales of (slot, head).  Every lane of the warp takes part; `live` lanes store.
-template <int DH, bool WIDE>
-__device__ __forceinline__ void quant_store(uint8_t* pool, int64_t slot, int hkv, int head, int c, float (&a)[8],
-                                            float (&b)[8], bool live) {
+// Quantise a lane's two runs of 8 dims (chunks c and DH / 16 + c of 8; the 4 lanes of a run of 32 are neighbours) and
+// store codes and scales of a row.  Every lane of the warp takes part; `live` lanes store.  fp32 values, any of them
+// possibly NaN or out of range.
+template <int DH>
+__device__ void quant_store_any(const SlotRow<DH>& at, int c, float (&a)[8], float (&b)[8], bool live) {
   float ma = 0.f, mb = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -91,37 +132,76 @@ __device__ __forceinline__ void quant_store(uint8_t* pool, int64_t slot, int hkv
   }
   const uint32_t ba = fp4_scale_byte(ma), bb = fp4_scale_byte(mb);
   const float sa = fp4_scale_value(ba), sb = fp4_scale_value(bb);
-  const float ia = ba ? 1.f / sa : 0.f, ib = bb ? 1.f / sb : 0.f;
+  float ha, la, hb, lb;
+  fp4_reciprocal(sa, ha, la);
+  fp4_reciprocal(sb, hb, lb);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    a[i] = ba ? fp4_quotient<WIDE>(a[i], sa, ia) : copysignf(0.f, a[i]);
-    b[i] = bb ? fp4_quotient<WIDE>(b[i], sb, ib) : copysignf(0.f, b[i]);
+    a[i] = fp4_quotient_32(a[i], sa, ha, la);
+    b[i] = fp4_quotient_32(b[i], sb, hb, lb);
   }
-  if (!live) return;
-  constexpr int HALF = DH / 16;  // chunks of 8 in half a head
-  const int t = static_cast<int>(slot % kBlockSize);
-  uint8_t* rec = pool + (slot / kBlockSize * hkv + head) * static_cast<int64_t>(Fp4<DH>::kRecord);
-  uint32_t* row = reinterpret_cast<uint32_t*>(rec + t * Fp4<DH>::kRow);
-  row[c] = fp4_pack8(a);
-  row[HALF + c] = fp4_pack8(b);
-  if ((c & 3) == 0) {
-    rec[Fp4<DH>::kScales + fp4_scale_at(c / 4, t)] = static_cast<uint8_t>(ba);
-    rec[Fp4<DH>::kScales + fp4_scale_at((HALF + c) / 4, t)] = static_cast<uint8_t>(bb);
+  if (live) store_codes<DH>(at, c, fp4_pack8(a), fp4_pack8(b), ba, bb);
+}
+
+template <int DT, int DH>
+__device__ __forceinline__ void quant_store(const SlotRow<DH>& at, int c, const Run8<DT>& ra, const Run8<DT>& rb, bool live) {
+  float a[8], b[8];
+  if constexpr (DT == MLB_F32) {
+    ra.get(a);
+    rb.get(b);
+    quant_store_any<DH>(at, c, a, b, live);
+  } else {
+    // the largest magnitudes as integers, two at a time (the order of positive fp16 / bf16 is that of their bits, NaN
+    // above all), then both runs' in one word through the two shuffles
+    uint32_t ma = 0u, mb = 0u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      ma = __vmaxu2(ma, ra.w[i] & 0x7fff7fffu);
+      mb = __vmaxu2(mb, rb.w[i] & 0x7fff7fffu);
+    }
+    uint32_t m = __vmaxu2(__byte_perm(ma, mb, 0x5410), __byte_perm(ma, mb, 0x7632));  // low: run a, high: run b
+    m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    constexpr uint32_t kTop = DT == MLB_BF16 ? 0x4770u : 0x7b80u;  // 61440
+    ra.get(a);
+    rb.get(b);
+    if (__any_sync(0xffffffffu, (m & 0xffffu) > kTop || (m >> 16) > kTop)) {  // NaN, infinity or a large value
+      quant_store_any<DH>(at, c, a, b, live);
+      return;
+    }
+    float fa, fb;
+    if constexpr (DT == MLB_BF16) {
+      fa = __uint_as_float(m << 16);
+      fb = __uint_as_float(m & 0xffff0000u);
+    } else {
+      fa = __half2float(__ushort_as_half(static_cast<unsigned short>(m)));
+      fb = __half2float(__ushort_as_half(static_cast<unsigned short>(m >> 16)));
+    }
+    const uint32_t ba = fp4_scale_byte_16(fa), bb = fp4_scale_byte_16(fb);
+    float ha, la, hb, lb;
+    fp4_reciprocal(fp4_scale_value(ba), ha, la);
+    fp4_reciprocal(fp4_scale_value(bb), hb, lb);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      a[i] = fp4_quotient_16(a[i], ha, la);
+      b[i] = fp4_quotient_16(b[i], hb, lb);
+    }
+    if (live) store_codes<DH>(at, c, fp4_pack8(a), fp4_pack8(b), ba, bb);
   }
 }
 
-// One warp per (token, group of 32 / LANES heads), grid-stride over `reps` groups of a token so that its row of
-// the table is read once for several groups.  Heads [0, h) are queries, [h, h + hkv) keys and, with APPEND,
-// [h + hkv, h + 2 hkv) values.
-template <int DT, int DH, bool APPEND>
-__global__ void __launch_bounds__(128) norm_rope_kernel(const RowArgs a, int groups, int reps, int tasks_per_token) {
+// One warp per (token, group of 32 / LANES heads of one kind: queries, keys or, with APPEND, values), over `reps`
+// groups of a token so that its row of the table is read once for several groups.
+template <int DT, int DH, bool APPEND, bool VEC>
+__global__ void __launch_bounds__(128) norm_rope_kernel(const RowArgs a, int reps, int tasks_per_token) {
   constexpr int LANES = DH / 16, PER = 32 / LANES, EB = Elt<DT>::bytes;
   griddep_begin();
   const int lane = threadIdx.x & 31, c = lane % LANES;
-  const int64_t task = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
-  const int64_t tok = task / tasks_per_token;
+  const uint32_t task = (blockIdx.x * blockDim.x + threadIdx.x) >> 5;  // at most 2^31 threads a launch
+  const int64_t tok = task / static_cast<uint32_t>(tasks_per_token);
   if (tok >= a.num_tokens) return;
-  const int g0 = static_cast<int>(task % tasks_per_token) * reps;
+  const int gq = (a.h + PER - 1) / PER, gk = (a.hkv + PER - 1) / PER, groups = gq + (APPEND ? 2 : 1) * gk;
+  const int g0 = static_cast<int>(task % static_cast<uint32_t>(tasks_per_token)) * reps, g_end = min(g0 + reps, groups);
   const int64_t pos = a.positions[tok];
   int64_t slot = 0;
   if constexpr (APPEND) slot = a.slots[tok];
@@ -136,163 +216,199 @@ __global__ void __launch_bounds__(128) norm_rope_kernel(const RowArgs a, int gro
   const bool turn = c < a.rot / 16;
   const int da = turn ? 8 * c : a.rot + 16 * (c - a.rot / 16);
   const int db = turn ? a.rot / 2 + 8 * c : da + 8;
-  float cs[8], sn[8];
-  if (turn) {
+  Run8<MLB_F32> cs, sn;
+  if (turn && g0 < gq + gk) {
     const char* row = reinterpret_cast<const char*>(a.cos_sin + pos * a.rot + 8 * c);
-    load8<MLB_F32>(row, true, cs);
-    load8<MLB_F32>(row + a.rot / 2 * 4, true, sn);
+    cs.load<true>(row);
+    sn.load<true>(row + a.rot / 2 * 4);
+  } else {
+    cs.zero();
+    sn.zero();
   }
-  for (int g = g0; g < g0 + reps && g < groups; ++g) {
-    const int head = g * PER + lane / LANES;
-    const bool is_q = head < a.h, is_k = !is_q && head < a.h + a.hkv;
-    const bool live = is_q || is_k || (APPEND && head < a.h + 2 * a.hkv);
-    const int kv_head = is_k ? head - a.h : head - a.h - a.hkv;
-    float xa[8], xb[8];
-    const char* src = is_q   ? a.q + (tok * a.q_st + head * a.q_sh) * EB
-                      : is_k ? a.k + (tok * a.k_st + kv_head * a.k_sh) * EB
-                             : a.v + (tok * a.v_st + kv_head * a.v_sh) * EB;
+  for (int g = g0; g < g_end; ++g) {
+    const int kind = g < gq ? 0 : !APPEND || g < gq + gk ? 1 : 2;  // uniform: the same for the whole warp
+    const int head = (g - (kind == 0 ? 0 : kind == 1 ? gq : gq + gk)) * PER + lane / LANES;
+    const bool live = head < (kind == 0 ? a.h : a.hkv);
+    const char* src = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
+    const int64_t st = kind == 0 ? a.q_st : kind == 1 ? a.k_st : a.v_st;
+    const int64_t sh = kind == 0 ? a.q_sh : kind == 1 ? a.k_sh : a.v_sh;
+    Run8<DT> ra, rb;
     if (live) {
-      load8<DT>(src + da * EB, a.vec, xa);
-      load8<DT>(src + db * EB, a.vec, xb);
+      src += (tok * st + head * sh) * EB;
+      ra.template load<VEC>(src + da * EB);
+      rb.template load<VEC>(src + db * EB);
     } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) xa[i] = xb[i] = 0.f;
+      ra.zero();
+      rb.zero();
     }
-    const char* weight = is_q ? a.q_weight : is_k ? a.k_weight : nullptr;
-    if (a.q_weight || a.k_weight) {  // uniform: the shuffles below are reached by every lane
-      float ss = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) ss = fmaf(xa[i], xa[i], fmaf(xb[i], xb[i], ss));
-#pragma unroll
-      for (int off = 1; off < LANES; off <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
+    if (kind < 2) {  // values pass as they are
+      float xa[8], xb[8];
+      ra.get(xa);
+      rb.get(xb);
+      const char* weight = kind == 0 ? a.q_weight : a.k_weight;
       if (weight) {
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss = fmaf(xa[i], xa[i], fmaf(xb[i], xb[i], ss));
+#pragma unroll
+        for (int off = 1; off < LANES; off <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
         const float r = rsqrtf(ss * (1.f / DH) + a.eps);
-        float wa[8], wb[8];
-        load8<DT>(weight + da * EB, true, wa);
-        load8<DT>(weight + db * EB, true, wb);
+        Run8<DT> w;
+        float f[8];
+        w.template load<true>(weight + da * EB);
+        w.get(f);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) xa[i] = xa[i] * r * wa[i], xb[i] = xb[i] * r * wb[i];
-      }
-    }
-    if (turn && (is_q || is_k)) {  // products rounded one by one, as the formula reads
+        for (int i = 0; i < 8; ++i) xa[i] = xa[i] * r * f[i];
+        w.template load<true>(weight + db * EB);
+        w.get(f);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float p = __fsub_rn(__fmul_rn(xa[i], cs[i]), __fmul_rn(xb[i], sn[i]));
-        xb[i] = __fadd_rn(__fmul_rn(xb[i], cs[i]), __fmul_rn(xa[i], sn[i]));
-        xa[i] = p;
+        for (int i = 0; i < 8; ++i) xb[i] = xb[i] * r * f[i];
       }
-    }
-    if (is_q || (!APPEND && is_k)) {
-      char* dst = is_q ? a.q_out + (tok * a.qo_st + head * a.qo_sh) * EB
-                       : a.k_out + (tok * a.ko_st + kv_head * a.ko_sh) * EB;
-      store8<DT>(dst + da * EB, a.vec, xa);
-      store8<DT>(dst + db * EB, a.vec, xb);
+      if (turn) {  // products rounded one by one, as the formula reads
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float co = __uint_as_float(cs.w[i]), si = __uint_as_float(sn.w[i]);
+          const float p = __fsub_rn(__fmul_rn(xa[i], co), __fmul_rn(xb[i], si));
+          xb[i] = __fadd_rn(__fmul_rn(xb[i], co), __fmul_rn(xa[i], si));
+          xa[i] = p;
+        }
+      }
+      ra.set(xa);  // a key's rounding to its own dtype, as when the two calls are made one by one
+      rb.set(xb);
+      if (live && (kind == 0 || !APPEND)) {
+        char* dst = kind == 0 ? a.q_out + (tok * a.qo_st + head * a.qo_sh) * EB
+                              : a.k_out + (tok * a.ko_st + head * a.ko_sh) * EB;
+        ra.template store<VEC>(dst + da * EB);
+        rb.template store<VEC>(dst + db * EB);
+      }
     }
     if constexpr (APPEND) {
-      // any lane of the warp with a key or value: all of them enter (shuffles inside)
-      if (g * PER + PER > a.h) {
-        if (is_k) {  // the key is rounded to its own dtype first, as when the two calls are made one by one
-#pragma unroll
-          for (int i = 0; i < 8; ++i) xa[i] = round_to<DT>(xa[i]), xb[i] = round_to<DT>(xb[i]);
-        }
-        quant_store<DH, DT == MLB_F32>(is_k ? a.k_cache : a.v_cache, slot, a.hkv, kv_head, c, xa, xb,
-                                       live && !is_q && slot_ok);
-      }
+      if (kind > 0)
+        quant_store<DT, DH>(SlotRow<DH>(kind == 1 ? a.k_cache : a.v_cache, slot_ok ? slot : 0, a.hkv, live ? head : 0), c,
+                            ra, rb, live && slot_ok);
     }
   }
 }
 
-// One group of Dh / 16 lanes per (token, head, K or V) row.
-template <int DT, int DH>
+// One group of Dh / 16 lanes per (token, head): its K row and its V row, which lie at the same place of their pools.
+template <int DT, int DH, bool VEC>
 __global__ void __launch_bounds__(128) fp4_append_kernel(const RowArgs a) {
   constexpr int LANES = DH / 16, EB = Elt<DT>::bytes;
   griddep_begin();
   const int lane = threadIdx.x & 31, c = lane % LANES;
-  const int64_t rows = a.num_tokens * a.hkv * 2;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x / LANES;
-  // every lane of a warp makes the same number of turns (shuffles inside)
-  const int64_t first = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x - lane) / LANES;
-  for (int64_t r0 = first; r0 < rows; r0 += step) {
-    const int64_t r = r0 + lane / LANES;
-    const bool live = r < rows;
-    const int64_t tok = live ? r / (2 * a.hkv) : 0;
-    const int which = static_cast<int>(live ? r % (2 * a.hkv) : 0), head = which % a.hkv;
-    const bool is_v = which >= a.hkv;
-    float xa[8], xb[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) xa[i] = xb[i] = 0.f;
-    int64_t slot = -1;
-    if (live) {
-      slot = a.slots[tok];
-      const char* src = is_v ? a.v + (tok * a.v_st + head * a.v_sh) * EB : a.k + (tok * a.k_st + head * a.k_sh) * EB;
-      load8<DT>(src + 8 * c * EB, a.vec, xa);
-      load8<DT>(src + (DH / 2 + 8 * c) * EB, a.vec, xb);
-    }
-    const bool ok = slot >= 0 && slot < a.num_slots;
-    if (live && !ok && which == 0 && c == 0) flag_error(a.err, MLB_DEV_SLOT_RANGE);
-    quant_store<DH, DT == MLB_F32>(is_v ? a.v_cache : a.k_cache, slot, a.hkv, head, c, xa, xb, ok);
+  const uint32_t hkv = static_cast<uint32_t>(a.hkv);
+  const uint32_t row = (blockIdx.x * blockDim.x + threadIdx.x) / LANES;  // at most 2^31 threads a launch
+  const bool in = row < static_cast<uint32_t>(a.num_tokens) * hkv;
+  const uint32_t tok = in ? row / hkv : 0;
+  const int head = static_cast<int>(in ? row - tok * hkv : 0);
+  Run8<DT> ka, kb, va, vb;
+  int64_t slot = -1;
+  if (in) {
+    slot = a.slots[tok];
+    const char* k = a.k + (tok * a.k_st + head * a.k_sh + 8 * c) * EB;
+    const char* v = a.v + (tok * a.v_st + head * a.v_sh + 8 * c) * EB;
+    ka.template load<VEC>(k);
+    kb.template load<VEC>(k + DH / 2 * EB);
+    va.template load<VEC>(v);
+    vb.template load<VEC>(v + DH / 2 * EB);
+  } else {
+    ka.zero();
+    kb.zero();
+    va.zero();
+    vb.zero();
   }
+  const bool ok = slot >= 0 && slot < a.num_slots;
+  if (in && !ok && head == 0 && c == 0) flag_error(a.err, MLB_DEV_SLOT_RANGE);
+  SlotRow<DH> at(a.k_cache, ok ? slot : 0, a.hkv, head);
+  quant_store<DT, DH>(at, c, ka, kb, ok);
+  at.rec += a.v_cache - a.k_cache;
+  quant_store<DT, DH>(at, c, va, vb, ok);
 }
 
-// Rows of slots as values: one group of Dh / 16 lanes per (token, head, K or V) row; a slot out of range reads 0.
+// Rows of slots as values: one group of Dh / 16 lanes per (token, head), its K row and its V row, two runs of
+// 8 dims each a lane (neighbouring lanes store neighbouring 16 bytes: with 16 dims in one run, every store filled half
+// of its 32-byte sectors and the kernel took 20 us instead of 13); a slot out of range reads 0.
 template <int DT, int DH>
 __global__ void __launch_bounds__(128) fp4_read_kernel(const RowArgs a) {
   constexpr int LANES = DH / 16, EB = Elt<DT>::bytes;
   griddep_begin();
-  const int64_t rows = a.num_tokens * a.hkv * 2;
-  const int64_t at = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / LANES;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x / LANES;
+  const uint32_t hkv = static_cast<uint32_t>(a.hkv);
+  const uint32_t row = (blockIdx.x * blockDim.x + threadIdx.x) / LANES;  // at most 2^31 threads a launch
+  if (row >= static_cast<uint32_t>(a.num_tokens) * hkv) return;
   const int c = threadIdx.x % LANES;
-  for (int64_t r = at; r < rows; r += step) {
-    const int64_t tok = r / (2 * a.hkv);
-    const int which = static_cast<int>(r % (2 * a.hkv)), head = which % a.hkv;
-    const bool is_v = which >= a.hkv;
-    const int64_t slot = a.slots[tok];
-    float x[2][8] = {};
-    if (slot >= 0 && slot < a.num_slots) {
-      const int t = static_cast<int>(slot % kBlockSize);
-      const uint8_t* rec = (is_v ? a.v_cache : a.k_cache) +
-                           (slot / kBlockSize * a.hkv + head) * static_cast<int64_t>(Fp4<DH>::kRecord);
-      const uint2 w = *reinterpret_cast<const uint2*>(rec + t * Fp4<DH>::kRow + 8 * c);  // dims [16c, 16c + 16)
-      const float s = fp4_scale_value(rec[Fp4<DH>::kScales + fp4_scale_at(c / 2, t)]);
+  const uint32_t tok = row / hkv;
+  const int head = static_cast<int>(row - tok * hkv);
+  const int64_t slot = a.slots[tok];
+  uint32_t w[2][2] = {}, scale[2][2] = {};  // [K, V][this lane's two runs of 8 dims]
+  if (slot >= 0 && slot < a.num_slots) {
+    const SlotRow<DH> at(a.k_cache, slot, a.hkv, head);
+    const int64_t to_v = a.v_cache - a.k_cache;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        uint32_t p[4];
-        fp4_unpack8(i ? w.y : w.x, p[0], p[1], p[2], p[3]);
+    for (int i = 0; i < 2; ++i) {
+      const uint8_t* codes = at.rec + at.t * Fp4<DH>::kRow + 4 * (i * LANES + c);
+      const uint8_t* s = at.rec + Fp4<DH>::kScales + fp4_scale_at((i * LANES + c) / 4, at.t);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p[j]));
-          x[i][2 * j] = f.x * s;
-          x[i][2 * j + 1] = f.y * s;
-        }
+      for (int kv = 0; kv < 2; ++kv) {
+        w[kv][i] = *reinterpret_cast<const uint32_t*>(codes + (kv ? to_v : 0));
+        scale[kv][i] = s[kv ? to_v : 0];
       }
-    } else if (which == 0 && c == 0) {
-      flag_error(a.err, MLB_DEV_SLOT_RANGE);
     }
-    char* dst = (is_v ? a.q_out : a.k_out) + ((tok * a.hkv + head) * DH + 16 * c) * EB;
-    store8<DT>(dst, true, x[0]);
-    store8<DT>(dst + 8 * EB, true, x[1]);
+  } else if (head == 0 && c == 0) {
+    flag_error(a.err, MLB_DEV_SLOT_RANGE);
+  }
+  const int64_t dst = (static_cast<int64_t>(row) * DH + 8 * c) * EB;
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t s2 = scale[kv][i] * 0x00010001u << 7;
+      Run8<MLB_F16> h;  // code * scale is exact in fp16 (and the wider types)
+      fp4_unpack8(w[kv][i], h.w[0], h.w[1], h.w[2], h.w[3]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) h.w[j] = hmul2_u32(h.w[j], s2);
+      char* to = (kv ? a.q_out : a.k_out) + dst + i * (DH / 2) * EB;
+      if constexpr (DT == MLB_F16) {
+        h.template store<true>(to);
+      } else {
+        float x[8];
+        h.get(x);
+        Run8<DT> r;
+        r.set(x);
+        r.template store<true>(to);
+      }
+    }
   }
 }
 
 template <int DT, int DH>
 cudaError_t launch_norm_rope_typed(const RowArgs& a, bool append, int num_sms, cudaStream_t s) {
   constexpr int PER = 32 / (DH / 16);
-  const int heads = a.h + (append ? 2 : 1) * a.hkv;
-  const int groups = (heads + PER - 1) / PER;
-  // a warp takes as many groups of a token as still leaves 16 warps on every SM
+  const int groups = (a.h + PER - 1) / PER + (append ? 2 : 1) * ((a.hkv + PER - 1) / PER);
+  // a warp takes as many groups of a token as still leaves 16 warps for every SM (8192 tokens of 32 + 8 heads: 31 us,
+  // with 64 warps 37)
   const int64_t warps = std::max<int64_t>(1, static_cast<int64_t>(num_sms) * 16);
   const int reps = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(groups, a.num_tokens * groups / warps)));
   const int tasks = (groups + reps - 1) / reps;
   const int64_t ctas = (a.num_tokens * tasks + 3) / 4;
   if (ctas > INT32_MAX) return cudaErrorInvalidValue;
-  if (append) return launch_k(norm_rope_kernel<DT, DH, true>, dim3(static_cast<unsigned>(ctas)), dim3(128), 0, s, a, groups, reps, tasks);
-  return launch_k(norm_rope_kernel<DT, DH, false>, dim3(static_cast<unsigned>(ctas)), dim3(128), 0, s, a, groups, reps, tasks);
+  const dim3 grid(static_cast<unsigned>(ctas)), block(128);
+  if (append)
+    return a.vec ? launch_k(norm_rope_kernel<DT, DH, true, true>, grid, block, 0, s, a, reps, tasks)
+                 : launch_k(norm_rope_kernel<DT, DH, true, false>, grid, block, 0, s, a, reps, tasks);
+  return a.vec ? launch_k(norm_rope_kernel<DT, DH, false, true>, grid, block, 0, s, a, reps, tasks)
+               : launch_k(norm_rope_kernel<DT, DH, false, false>, grid, block, 0, s, a, reps, tasks);
 }
 
-unsigned row_grid(const RowArgs& a, int dh, int num_sms) {
-  const int64_t threads = a.num_tokens * a.hkv * 2 * (dh / 16);
-  return static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>((threads + 127) / 128, static_cast<int64_t>(num_sms) * 64)));
+// one lane group per (token, head)
+unsigned row_grid(const RowArgs& a, int dh) {
+  return static_cast<unsigned>((a.num_tokens * a.hkv * (dh / 16) + 127) / 128);
+}
+
+template <int DT, int DH>
+cudaError_t launch_append_typed(const RowArgs& a, cudaStream_t s) {
+  const dim3 grid(row_grid(a, DH)), block(128);
+  return a.vec ? launch_k(fp4_append_kernel<DT, DH, true>, grid, block, 0, s, a)
+               : launch_k(fp4_append_kernel<DT, DH, false>, grid, block, 0, s, a);
 }
 
 }  // namespace
@@ -319,14 +435,14 @@ cudaError_t launch_norm_rope(const RowArgs& a, int dtype, int dh, bool append, i
 #undef MLB_CALL
 }
 
-cudaError_t launch_fp4_append(const RowArgs& a, int dtype, int dh, int num_sms, cudaStream_t s) {
-#define MLB_CALL(T, D) launch_k(fp4_append_kernel<T, D>, dim3(row_grid(a, dh, num_sms)), dim3(128), 0, s, a)
+cudaError_t launch_fp4_append(const RowArgs& a, int dtype, int dh, cudaStream_t s) {
+#define MLB_CALL(T, D) launch_append_typed<T, D>(a, s)
   MLB_FP4_DISPATCH(MLB_CALL)
 #undef MLB_CALL
 }
 
-cudaError_t launch_fp4_read(const RowArgs& a, int dtype, int dh, int num_sms, cudaStream_t s) {
-#define MLB_CALL(T, D) launch_k(fp4_read_kernel<T, D>, dim3(row_grid(a, dh, num_sms)), dim3(128), 0, s, a)
+cudaError_t launch_fp4_read(const RowArgs& a, int dtype, int dh, cudaStream_t s) {
+#define MLB_CALL(T, D) launch_k(fp4_read_kernel<T, D>, dim3(row_grid(a, D)), dim3(128), 0, s, a)
   MLB_FP4_DISPATCH(MLB_CALL)
 #undef MLB_CALL
 }
