@@ -891,8 +891,8 @@ int row_shapes(const char* what, int dtype, int64_t num_tokens, int num_heads, i
   if (num_tokens < 0 || num_heads < 0 || num_kv_heads < 0 || num_heads + num_kv_heads <= 0)
     return fail(MLB_EINVAL, "%s: bad sizes", what);
   if (!fp4_head_dim(head_dim)) return fail(MLB_EUNSUPPORTED, "%s: head_dim %d (supported: 64, 128, 256)", what, head_dim);
-  // thread indexes are 32-bit: head_dim / 16 threads a row, a warp at least a token
-  const int64_t threads = (static_cast<int64_t>(num_heads) + 2 * static_cast<int64_t>(num_kv_heads)) * (head_dim / 16) + 32;
+  // thread indexes are 32-bit: head_dim / 16 threads a row, whole warps for each of queries, keys and values
+  const int64_t threads = (static_cast<int64_t>(num_heads) + 2 * static_cast<int64_t>(num_kv_heads)) * (head_dim / 16) + 96;
   if (num_tokens > (int64_t(1) << 31) / threads)
     return fail(MLB_EINVAL, "%s: %lld tokens of %d heads are too many rows for one launch", what,
                 static_cast<long long>(num_tokens), num_heads + 2 * num_kv_heads);

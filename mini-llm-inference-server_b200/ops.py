@@ -116,6 +116,8 @@ class AttentionPlan:
     reduce_chunks_host: np.ndarray  # [N] pieces per token on the host
     has_query_tiles: bool = False  # kind-1 shared units (rows of >= 16 new tokens) in the plan
     max_pieces: int = 0  # the most pieces of one token
+    num_seqs: int = 0
+    max_blocks: int = 0  # width of the block tables it was planned for
 
 
 def _i32(a) -> np.ndarray:
@@ -174,7 +176,7 @@ def plan_attention(qo_indptr: list[int], seq_lens: list[int], max_blocks: int, n
                          max(1, 8 // (num_heads // num_kv_heads)), num_heads, num_kv_heads, n_tok,
                          units[:u].copy(), shared[:sh].copy(), members[:m].copy(), rows[:n_tok].copy(),
                          chunks[:n_tok].copy(), bool(sh and ((shared[:sh, 6] & 0xFF) == 1).any()),
-                         int(chunks[:n_tok].max()) if n_tok else 0)
+                         int(chunks[:n_tok].max()) if n_tok else 0, s, max_blocks)
 
 
 class Workspace:
@@ -490,12 +492,17 @@ def attention_partials_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     dev, shape, qs, code = q.get_device(), q.shape, q.stride(), DTYPE_CODE.get(q.dtype)
     if not (len(shape) == 3 and shape[2] == dh and qs[2] == 1 and (code == _lib.MLB_F16 or code == _lib.MLB_BF16)
             and dev == k_cache.get_device() and plan.num_tokens == shape[0] and plan.num_heads == shape[1]
-            and plan.num_kv_heads == hkv):
+            and plan.num_kv_heads == hkv and block_tables.dim() == 2 and block_tables.shape[0] == plan.num_seqs
+            and block_tables.shape[1] >= plan.max_blocks
+            and seq_lens.shape[0] == plan.num_seqs and qo_indptr.shape[0] == plan.num_seqs + 1):
         if len(shape) != 3 or shape[2] != dh or (shape[0] and qs[2] != 1):
             raise ValueError(f"{what}: q must be [N, H, {dh}] with unit last stride, got {tuple(q.shape)}")
         if q.dtype is not torch.bfloat16 and q.dtype is not torch.float16:
             raise ValueError(f"{what}: q must be float16 or bfloat16, got {q.dtype}")
-        if (plan.num_heads, plan.num_kv_heads, plan.num_tokens) != (shape[1], hkv, shape[0]):
+        if ((plan.num_heads, plan.num_kv_heads, plan.num_tokens) != (shape[1], hkv, shape[0])
+                or block_tables.dim() != 2 or block_tables.shape[0] != plan.num_seqs
+                or block_tables.shape[1] < plan.max_blocks
+                or tuple(seq_lens.shape) != (plan.num_seqs,) or tuple(qo_indptr.shape) != (plan.num_seqs + 1,)):
             raise ValueError(f"{what}: the plan was built for another shape")
         if q.device != k_cache.device:
             raise ValueError(f"{what}: q must be on the pools' device")
@@ -531,7 +538,8 @@ def paged_attention_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
                         scale: float | None = None, err: torch.Tensor | None = None,
                         targets: OutTargets | None = None) -> torch.Tensor | None:
     """`paged_attention` over 4-bit pools: q [N, H, Dh] float16 or bfloat16 -> [N, H, Dh] in q's dtype, the pools
-    holding this step's rows already (`kv_append_fp4`).  Same metadata tensors, plan and workspace."""
+    holding this step's rows already (`kv_append_fp4`).  Same metadata tensors, plan and workspace (calls that may
+    overlap on the GPU need a workspace each)."""
     workspace = workspace or Workspace()
     out = attention_partials_fp4(q, k_cache, v_cache, block_tables, seq_lens, qo_indptr, plan, workspace, out, scale,
                                  err, targets)
@@ -631,7 +639,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, cos_
     one launch (mlb_qk_norm_rope): q [N, H, Dh], k [N, Hkv, Dh] -> the same shapes and dtype, computed in fp32.
     q and k may be views of a fused projection.  positions int64 [N] (AttentionMetadata.positions); cos_sin from
     `rotary_table`, its rot_dim at most Dh (the dims behind it are not rotated).  out = (q_out, k_out) may be
-    (q, k)."""
+    (q, k), else memory that overlaps neither.  Rows whose position is outside the table are left unwritten."""
     what = "qk_norm_rope"
     code = _check_rope(what, q, k, positions, cos_sin, q_weight, k_weight)
     n, h, dh = q.shape

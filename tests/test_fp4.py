@@ -187,3 +187,37 @@ def test_attention_refusals(L):
                             (dict(kc=F + 1), L.MLB_EINVAL, "aligned"), (dict(nu=1 << 40), L.MLB_EINVAL, "grid")):
         assert attend(**bad) == code and word in L.last_error(), bad
     assert attend(nu=0, q=None) == L.MLB_OK
+
+
+def test_wide_reduction_refusals(L):
+    lib = L.lib()
+
+    def reduce(po=F, n=4, h=8, dh=64, dt=2, tpt=2, out=F, rows=4):
+        return lib.mlb_splitk_reduce_wide(po, F, rows, F, F, tpt, n, h, dh, out, 512, 64, dt, None, None)
+
+    for bad, code, word in ((dict(po=None), L.MLB_EINVAL, "null"), (dict(dt=9), L.MLB_EINVAL, "dtype"),
+                            (dict(dh=96), L.MLB_EUNSUPPORTED, "head_dim"), (dict(tpt=0), L.MLB_EINVAL, "sizes"),
+                            (dict(n=-1), L.MLB_EINVAL, "sizes"), (dict(out=None), L.MLB_EINVAL, "null out"),
+                            (dict(n=1 << 40), L.MLB_EINVAL, "grid")):
+        assert reduce(**bad) == code and word in L.last_error(), bad
+    assert reduce(n=0) == L.MLB_OK and reduce(rows=0) == L.MLB_OK
+
+
+def test_plan_for_4bit_pools(mlb):
+    """The split rule of 4-bit pools covers every page once, whatever it picks, and leaves other pools' plans alone."""
+    for lens, heads in (([1], (8, 2)), ([32001], (32, 8)), ([131072] * 16, (32, 8)), ([700, 5, 4096, 17] * 30, (28, 4)),
+                        ([1000000, 3], (8, 1))):
+        qo, width = list(range(len(lens) + 1)), -(-max(lens) // 16)
+        plan = mlb.plan_attention(qo, lens, width, *heads, "cpu", pool_dtype=torch.uint8)
+        seen = {}
+        for seq, _, begin, end, *_ in plan.units_host.tolist():
+            assert 0 <= begin < end <= -(-lens[seq] // 16)
+            seen.setdefault(seq, []).append((begin, end))
+        for s, n in enumerate(lens):
+            runs = sorted(seen[s])
+            assert runs[0][0] == 0 and runs[-1][1] == -(-n // 16)
+            assert all(a[1] == b[0] for a, b in zip(runs, runs[1:]))
+            assert plan.reduce_chunks_host[s] == len(runs)
+        assert plan.max_pieces == plan.reduce_chunks_host.max()
+        plain, half = (mlb.plan_attention(qo, lens, width, *heads, "cpu", pool_dtype=d) for d in (None, torch.bfloat16))
+        assert np.array_equal(plain.units_host, half.units_host)

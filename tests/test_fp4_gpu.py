@@ -251,6 +251,16 @@ def test_attention(mlb, cuda, heads, rows, dtype):
     assert int(err.item()) == 0
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads", [(32, 8, 128), (8, 2, 64), (8, 1, 128), (4, 4, 64)], ids=lambda h: "x".join(map(str, h)))
+def test_attention_of_long_chunks(mlb, cuda, heads, dtype):
+    """Query tiles over many key tiles (the rings of the tensor-core kernel turn over), whole and cut into pieces, odd
+    numbers of tiles, beside decode rows."""
+    st = Step(mlb, cuda, *heads, [(1500, 300), (0, 513), (2100, 17), (900, 1), (3000, 40)], dtype)
+    st.check(st.run(mlb, cuda))
+    st.check(st.run(mlb, cuda, pages=7))
+
+
 @pytest.mark.parametrize("heads", [(32, 8, 128), (8, 2, 64), (8, 8, 128), (6, 2, 256)], ids=lambda h: "x".join(map(str, h)))
 def test_attention_behind_a_shared_prefix(mlb, cuda, heads):
     steps = [(30 * 16 + 3 * i, 1) for i in range(40)] + [(30 * 16, 20)]
@@ -290,6 +300,48 @@ def test_attention_zero_and_nan_queries_stay_in_their_rows(mlb, cuda):
         got[1, 3] = want[1, 3]
         assert torch.equal(got, want)
     assert torch.equal(ref[2:], st.run(mlb, cuda)[2:])
+    st.q_dev[7, 0, 9] = float("nan")  # a row of a query tile
+    got = st.run(mlb, cuda)
+    assert got[7, 0].isnan().all() and got[7, 1:].isfinite().all() and torch.equal(got[8:], ref[8:])
+
+
+def test_refusals(mlb, cuda):
+    """What the GPU calls refuse: types, shapes, devices and strides they are not built for."""
+    st = Step(mlb, cuda, 8, 2, 64, [(20, 1), (3, 18)], torch.bfloat16)
+    m, plan, kp, vp, q = st.meta, st.plan(mlb, cuda), st.k_pool, st.v_pool, st.q_dev
+    good = dict(q=q, k_cache=kp, v_cache=vp, block_tables=m.block_tables_i32, seq_lens=m.seq_lens_i32,
+                qo_indptr=m.qo_indptr, plan=plan)
+    other = mlb.plan_attention([0, 19], [40], 3, 8, 2, cuda, pool_dtype=torch.uint8)  # as many tokens, another batch
+    for bad in (dict(q=q.float()), dict(q=q[:, :, :32]), dict(q=q.transpose(1, 2).contiguous().transpose(1, 2)), dict(q=q[:18]),
+                dict(q=q.cpu()), dict(k_cache=kp.to(torch.int16)), dict(k_cache=kp[:, :, :16]), dict(v_cache=vp[:5]),
+                dict(v_cache=vp.cpu()), dict(block_tables=m.block_tables), dict(block_tables=m.block_tables_i32[:, :1]),
+                dict(seq_lens=m.seq_lens_i32.cpu()), dict(plan=other), dict(out=torch.empty_like(q)[:18]),
+                dict(out=torch.empty_like(q, dtype=torch.float16)), dict(scale=0.0), dict(scale=-1.0)):
+        with pytest.raises(ValueError):
+            mlb.paged_attention_fp4(**{**good, **bad})
+    k, slots = torch.zeros(3, 2, 64, device=cuda), torch.arange(3, device=cuda)
+    for bad in (dict(k=k.to(torch.int32)), dict(k=k[:, :1]), dict(v=k[:2]), dict(v=k.half()), dict(slot_mapping=slots.int()),
+                dict(slot_mapping=slots[:2]), dict(slot_mapping=slots.cpu()), dict(k=k.cpu()), dict(k_cache=kp[::2]),
+                dict(k=k.transpose(1, 2).contiguous().transpose(1, 2))):
+        with pytest.raises(ValueError):
+            mlb.kv_append_fp4(**{**dict(k_cache=kp, v_cache=vp, slot_mapping=slots, k=k, v=k), **bad})
+    for bad in (dict(slot_mapping=slots[None]), dict(dtype=torch.int8), dict(slot_mapping=slots.float())):
+        with pytest.raises(ValueError):
+            mlb.kv_read_fp4(**{**dict(k_cache=kp, v_cache=vp, slot_mapping=slots), **bad})
+    table, w = torch.zeros(9, 64, device=cuda), torch.ones(64, device=cuda)
+    for bad in (dict(q=k.half()), dict(q=k[:2]), dict(q=k[:, :, :32]), dict(positions=slots.int()), dict(positions=slots[:2]),
+                dict(cos_sin=table.half()), dict(cos_sin=table[:, :40]), dict(cos_sin=table[:, ::2]), dict(q_weight=w[:32]),
+                dict(k_weight=w.half()), dict(k_weight=w.cpu()), dict(eps=-1.0), dict(out=(k[:2], k)),
+                dict(out=(k.half(), k)), dict(out=(k[:1].expand(3, 2, 64), k)), dict(cos_sin=torch.zeros(9, 24, device=cuda))):
+        with pytest.raises(ValueError):
+            mlb.qk_norm_rope(**{**dict(q=k, k=k, positions=slots, cos_sin=table), **bad})
+    ok = dict(q=k, k=k, v=k, positions=slots, cos_sin=table, k_cache=kp, v_cache=vp, slot_mapping=slots)
+    for bad in (dict(v=k[:2]), dict(v=k.half()), dict(slot_mapping=slots[:2]), dict(cos_sin=table[:, :32].contiguous()),
+                dict(k=k[:, :1], v=k[:, :1]), dict(out=k[:2])):
+        with pytest.raises(ValueError):
+            mlb.qk_norm_rope_append_fp4(**{**ok, **bad})
+    with pytest.raises(ValueError, match="block size"):
+        mlb.get_backend("b200").forward(q, k, k, kp, vp, mlb.AttentionMetadata.build([mlb.SeqStep(0, 19, [0])], 32, cuda))
 
 
 @pytest.mark.parametrize("tables", [True, False])
