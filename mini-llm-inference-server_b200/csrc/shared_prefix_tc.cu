@@ -265,7 +265,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const uint32_t k_smem = q_smem + L::kKOffset, v_smem = q_smem + L::kVOffset;
 
   griddep_begin();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // (the shuffle tells the compiler that the warp's index, and with it every branch on roles, is the warp's own)
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int kvh = blockIdx.x % a.hkv;
   // the CTA's pair of units: 2 * pair (tile A) and 2 * pair + 1 (tile B) share the page range, the table row
   // and the kind; a B without members leaves the CTA one tile
@@ -387,22 +388,46 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       // issued ahead of the softmax and P(j) . V_j -> S(j+2) runs while it works on tile j+1 (with two
       // buffers, S(j+1) queued behind P(j-1) . V and the softmax waited for it about a quarter of every
       // tile); o_done tells the softmax when the P . V products before its tile have completed.
-      if (lane == 0) {
+      if (elect_one()) {
+        // Descriptors of the 4-bit path: the address field counts 16 bytes and never carries into the fields above it
+        // (shared memory ends below 2^14 of them), so each is a base plus a constant.  (The 16-bit path has fewer
+        // registers here: the bases would spill, 730 us instead of 709 on 4 chunks of 1500..2000 tokens.)
+        const uint64_t q_desc = sw128_desc(q_smem, 16, 1024), k_desc = sw128_desc(k_smem, 16, 1024);
+        const uint64_t v_desc = sw128_desc(v_smem, kTcRows * 128, 1024);
         auto issue_s = [&](uint32_t s_col, int x, int j) {  // S = Q_x . K_j^T (K = Dh in steps of 16)
-          const uint32_t kb = k_smem + (j % NK) * L::kTileBytes, qx = q_smem + x * L::kQBytes;
+          if constexpr (FP4) {
+            const uint64_t qx = q_desc + static_cast<uint32_t>(x * (L::kQBytes >> 4));
+            const uint64_t kb = k_desc + static_cast<uint32_t>((j % NK) * (L::kTileBytes >> 4));
 #pragma unroll
-          for (int ks = 0; ks < DH / 16; ++ks) {
-            const uint32_t off = (ks >> 2) * (kTcRows * 128) + (ks & 3) * 32;
-            umma_ss(tmem + s_col, sw128_desc(qx + off, 16, 1024), sw128_desc(kb + off, 16, 1024), kIdescS,
-                    ks > 0 ? 1u : 0u);
+            for (int ks = 0; ks < DH / 16; ++ks) {
+              const uint32_t off = (ks >> 2) * ((kTcRows * 128) >> 4) + (ks & 3) * 2;
+              umma_ss(tmem + s_col, qx + off, kb + off, kIdescS, ks > 0 ? 1u : 0u);
+            }
+          } else {
+            const uint32_t kb = k_smem + (j % NK) * L::kTileBytes, qx = q_smem + x * L::kQBytes;
+#pragma unroll
+            for (int ks = 0; ks < DH / 16; ++ks) {
+              const uint32_t off = (ks >> 2) * (kTcRows * 128) + (ks & 3) * 32;
+              umma_ss(tmem + s_col, sw128_desc(qx + off, 16, 1024), sw128_desc(kb + off, 16, 1024), kIdescS,
+                      ks > 0 ? 1u : 0u);
+            }
           }
         };
         auto issue_pv = [&](uint32_t o_col, uint32_t p_col, int j) {  // O += P . V_j, one k-step per loaded page
-          const uint32_t vb = v_smem + (j % NV) * L::kTileBytes;
           const int live_pages = min(kTcTilePages, npages - j * kTcTilePages);
-          for (int ks = 0; ks < live_pages; ++ks)
-            umma_ts(tmem + o_col, tmem + p_col + ks * 8, sw128_desc(vb + ks * 16 * 128, kTcRows * 128, 1024),
-                    kIdescO, (j > 0 || ks > 0) ? 1u : 0u);
+          if constexpr (FP4) {
+            const uint64_t vb = v_desc + static_cast<uint32_t>((j % NV) * (L::kTileBytes >> 4));
+#pragma unroll
+            for (int ks = 0; ks < kTcTilePages; ++ks)
+              if (ks < live_pages)
+                umma_ts(tmem + o_col, tmem + p_col + ks * 8, vb + ks * ((16 * 128) >> 4), kIdescO,
+                        (j > 0 || ks > 0) ? 1u : 0u);
+          } else {
+            const uint32_t vb = v_smem + (j % NV) * L::kTileBytes;
+            for (int ks = 0; ks < live_pages; ++ks)
+              umma_ts(tmem + o_col, tmem + p_col + ks * 8, sw128_desc(vb + ks * 16 * 128, kTcRows * 128, 1024),
+                      kIdescO, (j > 0 || ks > 0) ? 1u : 0u);
+          }
         };
         auto wait_k = [&](int j) {
           if (!tc_wait(kfull + j % NK, (j / NK) & 1, abort_flag, a.err)) return false;

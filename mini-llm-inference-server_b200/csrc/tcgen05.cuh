@@ -47,6 +47,14 @@ __host__ __device__ constexpr uint32_t f16_idesc(uint32_t fmt, bool b_mn_major, 
          (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
 
+// One lane of a converged warp, in a form that lets the compiler keep what the lane computes in uniform registers (a
+// tcgen05.mma takes its operands from there; behind `lane == 0` each of them is moved over one by one).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n.reg .pred q;\nelect.sync _|q, 0xffffffff;\nselp.u32 %0, 1, 0, q;\n}\n" : "=r"(p));
+  return p != 0;
+}
+
 __device__ __forceinline__ void umma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                                         uint32_t accumulate) {
   asm volatile(
