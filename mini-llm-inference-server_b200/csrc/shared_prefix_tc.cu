@@ -103,6 +103,13 @@ struct TcLayout {
   static constexpr int kLaunchBytes = kBytes + 1024;  // slack to align the base to 1024 (swizzle atoms)
 };
 
+// the larger of three in one instruction (NaN is passed over, as by fmaxf)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 // Byte offset of 16-byte chunk c (of a DH x 2-byte row) of row r in a [DH/64][128][64] swizzled tile.
 __device__ __forceinline__ uint32_t sw_chunk(int r, int c) {
   return static_cast<uint32_t>((c >> 3) * (kTcRows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
@@ -631,7 +638,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
       for (int i = 0; i < 8; ++i) mx8[i] = __uint_as_float(sr[i]);
 #pragma unroll
-      for (int k = 8; k < kTcTileTokens; ++k) mx8[k % 8] = fmaxf(mx8[k % 8], __uint_as_float(sr[k]));
+      for (int k = 8; k < kTcTileTokens; k += 2)
+        mx8[k / 2 % 8] = max3(mx8[k / 2 % 8], __uint_as_float(sr[k]), __uint_as_float(sr[k + 1]));
       const float mraw = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])),
                                fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
       if (!FP4 && tile_unit && x == 0) {

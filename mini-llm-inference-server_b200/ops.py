@@ -180,19 +180,31 @@ def plan_attention(qo_indptr: list[int], seq_lens: list[int], max_blocks: int, n
 
 
 class Workspace:
-    """Split-K scratch (fp32 partial rows + their log-sum-exp), grown on demand and reused across calls."""
+    """Split-K scratch (fp32 partial rows + their log-sum-exp), grown on demand and reused across calls.  What it
+    has outgrown stays allocated as long as the workspace (a captured graph may hold its address); it grows by half
+    at least, so that all of it stays below three times the largest."""
 
     def __init__(self) -> None:
         self._o: torch.Tensor | None = None
         self._lse: torch.Tensor | None = None
+        self._held: list[tuple[torch.Tensor, torch.Tensor]] = []
 
     def get(self, rows: int, heads: int, dh: int, device: torch.device) -> tuple[torch.Tensor, torch.Tensor]:
         need_o, need_l = rows * heads * dh, rows * heads
-        if self._o is None or self._o.device != device or self._o.numel() < need_o:
-            self._o = torch.empty(max(need_o, 1), dtype=torch.float32, device=device)
-        if self._lse is None or self._lse.device != device or self._lse.numel() < need_l:
-            self._lse = torch.empty(max(need_l, 1), dtype=torch.float32, device=device)
+        if self._o is None or self._o.device != device or self._o.numel() < need_o or self._lse.numel() < need_l:
+            self._grow(need_o, need_l, device)
         return self._o, self._lse
+
+    def _grow(self, need_o: int, need_l: int, device: torch.device) -> None:
+        held = [(o, lse) for o, lse in self._held if o.device == device]
+        fits = [(o, lse) for o, lse in held if o.numel() >= need_o and lse.numel() >= need_l]
+        if not fits:
+            if held:
+                need_o, need_l = max(need_o, 3 * held[-1][0].numel() // 2), max(need_l, 3 * held[-1][1].numel() // 2)
+            fits = [(torch.empty(max(need_o, 1), dtype=torch.float32, device=device),
+                     torch.empty(max(need_l, 1), dtype=torch.float32, device=device))]
+            self._held += fits
+        self._o, self._lse = fits[-1]
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
@@ -494,7 +506,7 @@ def attention_partials_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
             and dev == k_cache.get_device() and plan.num_tokens == shape[0] and plan.num_heads == shape[1]
             and plan.num_kv_heads == hkv and block_tables.dim() == 2 and block_tables.shape[0] == plan.num_seqs
             and block_tables.shape[1] >= plan.max_blocks
-            and seq_lens.shape[0] == plan.num_seqs and qo_indptr.shape[0] == plan.num_seqs + 1):
+            and seq_lens.shape == (plan.num_seqs,) and qo_indptr.shape == (plan.num_seqs + 1,)):
         if len(shape) != 3 or shape[2] != dh or (shape[0] and qs[2] != 1):
             raise ValueError(f"{what}: q must be [N, H, {dh}] with unit last stride, got {tuple(q.shape)}")
         if q.dtype is not torch.bfloat16 and q.dtype is not torch.float16:

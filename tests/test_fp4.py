@@ -3,6 +3,7 @@ entry points (every call here is refused, or has nothing to do, before a launch)
 
 from __future__ import annotations
 
+import weakref
 from importlib import import_module
 
 import numpy as np
@@ -221,3 +222,17 @@ def test_plan_for_4bit_pools(mlb):
         assert plan.max_pieces == plan.reduce_chunks_host.max()
         plain, half = (mlb.plan_attention(qo, lens, width, *heads, "cpu", pool_dtype=d) for d in (None, torch.bfloat16))
         assert np.array_equal(plain.units_host, half.units_host)
+
+
+def test_workspace_keeps_what_it_has_outgrown(mlb):
+    """A captured graph may hold the address of a buffer that a later call found too small."""
+    ws, dev = mlb.Workspace(), torch.device("cpu")
+    first = ws.get(4, 2, 64, dev)
+    assert [t.numel() for t in first] == [512, 8] and ws.get(3, 2, 64, dev)[0] is first[0]
+    refs = [weakref.ref(t) for t in first]
+    del first
+    grown = ws.get(5, 2, 64, dev)
+    assert [t.numel() for t in grown] == [768, 12] and all(r() is not None for r in refs)
+    other = ws.get(9, 2, 64, torch.device("meta"))
+    assert other[0].device.type == "meta" and other[0].numel() == 9 * 2 * 64
+    assert ws.get(6, 2, 64, dev)[0] is grown[0]  # back on the first device: no new buffer

@@ -421,6 +421,25 @@ def test_attention_is_deterministic_and_captures(mlb, cuda):
     assert torch.equal(outs[0], want)
 
 
+def test_a_grown_workspace_leaves_a_captured_graph_its_buffer(mlb, cuda):
+    st = Step(mlb, cuda, 8, 2, 128, [(3000, 1), (500, 1)], torch.float16)
+    ws, m = mlb.Workspace(), st.meta
+    plan = st.plan(mlb, cuda)
+    assert plan.num_partial_rows
+    run = lambda: mlb.paged_attention_fp4(st.q_dev, st.k_pool, st.v_pool, m.block_tables_i32, m.seq_lens_i32,  # noqa: E731
+                                          m.qo_indptr, plan, ws)
+    ref = run()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = run()
+    rows = plan.num_partial_rows
+    ws.get(100 * rows, 8, 128, ref.device)
+    others = [torch.full((rows * 8 * 128,), float("nan"), device=cuda) for _ in range(8)]  # would take a freed buffer
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, ref) and all(x.isnan().all() for x in others)
+
+
 # ---------------------------------------------------------------- together
 
 
