@@ -473,6 +473,23 @@ MLB_API int mlb_splitk_reduce_wide(const float* partial_o, const float* partial_
                       void* out, int64_t out_stride_tok, int64_t out_stride_head, int out_dtype,
                       const mlb_out_targets* out_targets, void* stream);
 
+/*
+ * One of the entry points above with its arguments as 8-byte words, in their order: integers and pointers as they
+ * are, a float as the bits of a double.  The same checks, results and status; a wrong number of words or an int that
+ * does not fit is MLB_EINVAL.  For bindings that convert arguments one by one, where thirty of them cost more than
+ * the launch (ctypes: 7 us, as one packed string 2).
+ */
+enum {
+  MLB_CALL_KV_APPEND_FP4 = 1,
+  MLB_CALL_KV_READ_FP4 = 2,
+  MLB_CALL_QK_NORM_ROPE = 3,
+  MLB_CALL_QK_NORM_ROPE_APPEND_FP4 = 4,
+  MLB_CALL_PAGED_ATTENTION_FP4 = 5,
+  MLB_CALL_SPLITK_REDUCE = 6,
+  MLB_CALL_SPLITK_REDUCE_WIDE = 7
+};
+MLB_API int mlb_call_words(int entry, const int64_t* words, int num_words);
+
 #ifdef __cplusplus
 }
 #endif

@@ -7,7 +7,11 @@
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
+#include <cstring>
 #include <string>
+#include <tuple>
+#include <type_traits>
+#include <utility>
 #include <vector>
 
 #include "attn_args.cuh"
@@ -1100,4 +1104,53 @@ extern "C" int mlb_splitk_reduce_wide(const float* partial_o, const float* parti
                                                     num_tokens, num_heads, head_dim, targets, out_dtype,
                                                     static_cast<cudaStream_t>(stream)),
                      what);
+}
+
+// ---------------------------------------------------------------- calls by words
+
+namespace {
+
+// One argument out of its word; `ok` is cleared by an int that does not fit.
+template <class T>
+T from_word(int64_t w, bool& ok) {
+  if constexpr (std::is_pointer_v<T>) {
+    return reinterpret_cast<T>(static_cast<uintptr_t>(w));
+  } else if constexpr (std::is_floating_point_v<T>) {
+    double d;
+    std::memcpy(&d, &w, sizeof d);
+    return static_cast<T>(d);
+  } else {
+    if (static_cast<int64_t>(static_cast<T>(w)) != w) ok = false;
+    return static_cast<T>(w);
+  }
+}
+
+template <class... A, size_t... I>
+int call_with(const char* what, int (*fn)(A...), const int64_t* w, std::index_sequence<I...>) {
+  bool ok = true;
+  const std::tuple<A...> args{from_word<A>(w[I], ok)...};
+  if (!ok) return fail(MLB_EINVAL, "%s: an integer argument does not fit", what);
+  return std::apply(fn, args);
+}
+template <class... A>
+int call_words(const char* what, int (*fn)(A...), const int64_t* w, int n) {
+  if (!w || n != static_cast<int>(sizeof...(A)))
+    return fail(MLB_EINVAL, "%s: %d words for %d arguments", what, n, static_cast<int>(sizeof...(A)));
+  return call_with(what, fn, w, std::index_sequence_for<A...>{});
+}
+
+}  // namespace
+
+extern "C" int mlb_call_words(int entry, const int64_t* words, int num_words) {
+  switch (entry) {
+    case MLB_CALL_KV_APPEND_FP4: return call_words("kv_append_fp4", mlb_kv_append_fp4, words, num_words);
+    case MLB_CALL_KV_READ_FP4: return call_words("kv_read_fp4", mlb_kv_read_fp4, words, num_words);
+    case MLB_CALL_QK_NORM_ROPE: return call_words("qk_norm_rope", mlb_qk_norm_rope, words, num_words);
+    case MLB_CALL_QK_NORM_ROPE_APPEND_FP4:
+      return call_words("qk_norm_rope_append_fp4", mlb_qk_norm_rope_append_fp4, words, num_words);
+    case MLB_CALL_PAGED_ATTENTION_FP4: return call_words("paged_attention_fp4", mlb_paged_attention_fp4, words, num_words);
+    case MLB_CALL_SPLITK_REDUCE: return call_words("splitk_reduce", mlb_splitk_reduce, words, num_words);
+    case MLB_CALL_SPLITK_REDUCE_WIDE: return call_words("splitk_reduce_wide", mlb_splitk_reduce_wide, words, num_words);
+  }
+  return fail(MLB_EINVAL, "call_words: no entry %d", entry);
 }

@@ -406,15 +406,21 @@ def fp4_pool_shape(num_blocks: int, num_kv_heads: int, head_dim: int) -> tuple[i
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
-def _launch(fn, what: str, device: int, *args) -> None:
+def _launch(entry: _lib.Entry, what: str, device: int, *args) -> None:
     """Call an entry point with the current stream of `device` (an ordinal), made current if it is not already."""
     if _current_device() == device:
-        rc = fn(*args, _raw_stream(device) if _raw_stream else torch.cuda.current_stream(device).cuda_stream)
+        stream = _raw_stream(device) if _raw_stream else torch.cuda.current_stream(device).cuda_stream
+        rc = lib().mlb_call_words(entry.number, entry.pack(*args, stream), entry.num_words)
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+            stream = torch.cuda.current_stream(device).cuda_stream
+            rc = lib().mlb_call_words(entry.number, entry.pack(*args, stream), entry.num_words)
     if rc:
         check(rc, what)
+
+
+def _adr(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 # A decode step makes several of these calls per layer, each a few microseconds on the GPU: every entry point below
@@ -467,8 +473,8 @@ def kv_append_fp4(k_cache: torch.Tensor, v_cache: torch.Tensor, slot_mapping: to
         _check_index(slot_mapping, shape[0], k_cache.device, what, "slot_mapping")
         _code(k, what)
     if shape[0]:
-        _launch(lib().mlb_kv_append_fp4, what, dev, k_cache.data_ptr(), v_cache.data_ptr(), nb, slot_mapping.data_ptr(),
-                k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], code, shape[0], hkv, dh, _ptr(err))
+        _launch(_lib.KV_APPEND_FP4, what, dev, k_cache.data_ptr(), v_cache.data_ptr(), nb, slot_mapping.data_ptr(),
+                k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], code, shape[0], hkv, dh, _adr(err))
 
 
 def kv_read_fp4(k_cache: torch.Tensor, v_cache: torch.Tensor, slot_mapping: torch.Tensor,
@@ -488,8 +494,8 @@ def kv_read_fp4(k_cache: torch.Tensor, v_cache: torch.Tensor, slot_mapping: torc
     k = k_cache.new_empty((n, hkv, dh), dtype=dtype)
     v = torch.empty_like(k)
     if n:
-        _launch(lib().mlb_kv_read_fp4, what, dev, k_cache.data_ptr(), v_cache.data_ptr(), nb, slot_mapping.data_ptr(),
-                k.data_ptr(), v.data_ptr(), DTYPE_CODE[dtype], n, hkv, dh, _ptr(err))
+        _launch(_lib.KV_READ_FP4, what, dev, k_cache.data_ptr(), v_cache.data_ptr(), nb, slot_mapping.data_ptr(),
+                k.data_ptr(), v.data_ptr(), DTYPE_CODE[dtype], n, hkv, dh, _adr(err))
     return k, v
 
 
@@ -536,11 +542,12 @@ def attention_partials_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     po = plse = None
     if plan.num_partial_rows:
         po, plse = workspace.get(plan.num_partial_rows, h, dh, q.device)
-    _launch(lib().mlb_paged_attention_fp4, what, dev, q.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(),
+    _launch(_lib.PAGED_ATTENTION_FP4, what, dev, q.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(),
             code, nb, h, hkv, dh, 1.0 / math.sqrt(dh) if scale is None else float(scale), block_tables.data_ptr(),
             block_tables.stride(0), seq_lens.data_ptr(), qo_indptr.data_ptr(), seq_lens.shape[0], plan.units.data_ptr(),
-            plan.num_units, plan.shared_units.data_ptr(), plan.num_shared_units, plan.members.data_ptr(), _ptr(po),
-            _ptr(plse), plan.num_partial_rows, _ptr(out), o0, o1, _targets(targets), _ptr(err))
+            plan.num_units, plan.shared_units.data_ptr(), plan.num_shared_units, plan.members.data_ptr(), _adr(po),
+            _adr(plse), plan.num_partial_rows, _adr(out), o0, o1, 0 if targets is None else ctypes.addressof(targets),
+            _adr(err))
     return out
 
 
@@ -559,10 +566,10 @@ def paged_attention_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
         dev = q.get_device()
         po, plse = workspace.get(plan.num_partial_rows, plan.num_heads, q.shape[2], q.device)
         wide = plan.max_pieces > WIDE_REDUCE_PIECES
-        _launch(lib().mlb_splitk_reduce_wide if wide else lib().mlb_splitk_reduce, "splitk_reduce", dev, po.data_ptr(),
+        _launch(_lib.SPLITK_REDUCE_WIDE if wide else _lib.SPLITK_REDUCE, "splitk_reduce", dev, po.data_ptr(),
                 plse.data_ptr(), plan.num_partial_rows, plan.reduce_rows.data_ptr(), plan.reduce_chunks.data_ptr(),
-                plan.tokens_per_tile, plan.num_tokens, plan.num_heads, q.shape[2], _ptr(out), *_strides(out),
-                DTYPE_CODE[q.dtype], _targets(targets))
+                plan.tokens_per_tile, plan.num_tokens, plan.num_heads, q.shape[2], _adr(out), *_strides(out),
+                DTYPE_CODE[q.dtype], 0 if targets is None else ctypes.addressof(targets))
     return out
 
 
@@ -664,9 +671,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, cos_
         _check_row_out(what, ko, k)
     qs, ks, qos, kos = q.stride(), k.stride(), qo.stride(), ko.stride()
     rows, rot = cos_sin.shape
-    _launch(lib().mlb_qk_norm_rope, what, q.get_device(), q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], code,
-            n, h, k.shape[1], dh, positions.data_ptr(), cos_sin.data_ptr(), rows, rot, _ptr(q_weight), _ptr(k_weight),
-            eps, qo.data_ptr(), qos[0], qos[1], ko.data_ptr(), kos[0], kos[1], _ptr(err))
+    _launch(_lib.QK_NORM_ROPE, what, q.get_device(), q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], code,
+            n, h, k.shape[1], dh, positions.data_ptr(), cos_sin.data_ptr(), rows, rot, _adr(q_weight), _adr(k_weight),
+            eps, qo.data_ptr(), qos[0], qos[1], ko.data_ptr(), kos[0], kos[1], _adr(err))
     return qo, ko
 
 
@@ -696,10 +703,10 @@ def qk_norm_rope_append_fp4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, p
         _check_row_out(what, out, q)
     qs, os = q.stride(), out.stride()
     rows, rot = cos_sin.shape
-    _launch(lib().mlb_qk_norm_rope_append_fp4, what, dev, q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1],
+    _launch(_lib.QK_NORM_ROPE_APPEND_FP4, what, dev, q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1],
             v.data_ptr(), vs[0], vs[1], code, n, h, hkv, dh, positions.data_ptr(), cos_sin.data_ptr(), rows, rot,
-            _ptr(q_weight), _ptr(k_weight), eps, out.data_ptr(), os[0], os[1], k_cache.data_ptr(), v_cache.data_ptr(), nb,
-            slot_mapping.data_ptr(), _ptr(err))
+            _adr(q_weight), _adr(k_weight), eps, out.data_ptr(), os[0], os[1], k_cache.data_ptr(), v_cache.data_ptr(), nb,
+            slot_mapping.data_ptr(), _adr(err))
     return out
 
 

@@ -3,8 +3,10 @@ entry points (every call here is refused, or has nothing to do, before a launch)
 
 from __future__ import annotations
 
+import re
 import weakref
 from importlib import import_module
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -202,6 +204,28 @@ def test_wide_reduction_refusals(L):
                             (dict(n=1 << 40), L.MLB_EINVAL, "grid")):
         assert reduce(**bad) == code and word in L.last_error(), bad
     assert reduce(n=0) == L.MLB_OK and reduce(rows=0) == L.MLB_OK
+
+
+def test_calls_by_words(L):
+    """The numbers are the header's; counts and ints are checked; the entry point behind refuses as it does directly."""
+    header = (Path(__file__).parents[1] / "include" / "mlb_paged_kv.h").read_text()
+    numbers = {n: int(v) for n, v in re.findall(r"MLB_CALL_(\w+) = (\d+)", header)}
+    assert len(numbers) == 7 and all(getattr(L, n).number == v for n, v in numbers.items())
+    call, e = L.lib().mlb_call_words, L.KV_APPEND_FP4
+    args = [1 << 20, 1 << 20, 10, 64, 64, 1024, 128, 64, 1024, 128, 2, 0, 8, 128, 0, 0]
+    assert call(e.number, e.pack(*args), e.num_words) == L.MLB_OK  # no tokens: nothing to do
+    assert call(e.number, e.pack(*args), e.num_words - 1) == L.MLB_EINVAL and "15 words for 16" in L.last_error()
+    assert call(e.number, None, e.num_words) == L.MLB_EINVAL
+    assert call(99, e.pack(*args), e.num_words) == L.MLB_EINVAL and "99" in L.last_error()
+    wide = args[:12] + [8 + (1 << 32)] + args[13:]  # a head count that an int would cut to 8
+    assert call(e.number, e.pack(*wide), e.num_words) == L.MLB_EINVAL and "does not fit" in L.last_error()
+    bad = args[:13] + [96] + args[14:]
+    assert call(e.number, e.pack(*bad), e.num_words) == L.MLB_EUNSUPPORTED
+    words = L.last_error()
+    assert L.lib().mlb_kv_append_fp4(*bad) == L.MLB_EUNSUPPORTED and L.last_error() == words
+    r = L.QK_NORM_ROPE  # a float among the words
+    rope = [64, 0, 0, 64, 0, 0, 2, 1, 1, 1, 128, 64, 64, 8, 128, 0, 0, -1.0, 64, 0, 0, 64, 0, 0, 0, 0]
+    assert call(r.number, r.pack(*rope), r.num_words) == L.MLB_EINVAL and "eps" in L.last_error()
 
 
 def test_plan_for_4bit_pools(mlb):
