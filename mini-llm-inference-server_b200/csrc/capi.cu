@@ -506,8 +506,8 @@ int mlb_plan_attention(const int32_t* qo_indptr, const int32_t* seq_lens, int nu
   int64_t piece_pages = kPrefillPiecePages;
   if (pages_per_unit == MLB_PAGES_PER_UNIT_FP4) {
     // every piece costs a start, and its tokens' fp32 partial rows written and read again: rows are cut only as far
-    // as it takes to give every SM about 3 CTAs (4 rows of 1500..2000 new tokens, 4-bit pools: 882 us in pieces of
-    // 128 pages, 668 us whole)
+    // as it takes to give every SM about 3 CTAs (4 rows of 1500..2000 new tokens, 4-bit pools: 807 us in pieces of
+    // 128 pages, 589 us whole)
     int64_t work = 0;
     for (int s : prefill_seqs) {
       const int n = qo_indptr[s + 1] - qo_indptr[s], L = seq_lens[s];
