@@ -440,6 +440,49 @@ def test_a_grown_workspace_leaves_a_captured_graph_its_buffer(mlb, cuda):
     assert torch.equal(out, ref) and all(x.isnan().all() for x in others)
 
 
+@pytest.mark.parametrize("steps,shared", [([(3000, 1), (500, 1), (0, 40), (37, 16), (9, 3)], 0), ([(300 + i, 1) for i in range(9)], 16)])
+def test_attention_into_targets(mlb, cuda, steps, shared):
+    """Rows for several destinations, among other heads' rows, as KV-head sharding stores them."""
+    st = Step(mlb, cuda, 32, 8, 128, steps, torch.bfloat16, shared=shared)
+    ref, n = st.run(mlb, cuda), len(st.q)
+    bufs = [torch.full((n, 40, 128), float("nan"), dtype=torch.bfloat16, device=cuda) for _ in range(2)]
+    to = mlb.ops.out_targets([b.data_ptr() for b in bufs], 5, 40 * 128, 128)
+    assert st.run(mlb, cuda, targets=to) is None
+    for b in bufs:
+        assert torch.equal(b[:, 5:37], ref) and b[:, :5].isnan().all() and b[:, 37:].isnan().all()
+
+
+@pytest.mark.parametrize("exchange", ["packets", "barrier"])
+def test_backend_gathers_rows_of_a_4bit_cache(mlb, cuda, exchange):
+    """One rank of KV-head sharding's own transport (no peer to wait for): the rows of a plain forward."""
+    import torch.distributed as dist
+
+    sharding = __import__(mlb.__name__ + ".sharding", fromlist=["PeerOutputs"])
+    own_group = not dist.is_initialized()
+    if own_group:
+        dist.init_process_group("gloo", store=dist.HashStore(), rank=0, world_size=1)
+    try:
+        st = Step(mlb, cuda, 32, 8, 128, [(700, 1), (300, 1), (10, 40), (37, 5)], torch.bfloat16)
+        n, g = len(st.q), torch.Generator().manual_seed(4)
+        k, v = (torch.randn(n, 8, 128, generator=g).to(torch.bfloat16).to(cuda) for _ in range(2))
+        backend = mlb.get_backend("b200", check_errors=True, pages_per_unit=16)
+        pools = [(st.k_pool.clone(), st.v_pool.clone()) for _ in range(2)]
+        ref = backend.forward(st.q_dev, k, v, *pools[0], st.meta)
+        plan = backend.plan(st.meta, 32, 8, st.q_dev.device, torch.uint8)
+        assert 1 < plan.max_pieces <= mlb.ops.WIDE_REDUCE_PIECES  # one reduction's order of sums on both sides
+        peers = sharding.PeerOutputs(n + 3, 32, 128, torch.bfloat16, cuda, slots=2, exchange=exchange)
+        for slot in (0, 1):
+            peers.output(slot, n).fill_(float("nan"))
+            assert backend.forward(st.q_dev, k, v, *pools[1], st.meta, peer_gather=(peers, slot, 0)) is None
+            assert torch.equal(peers.output(slot, n), ref)
+        assert torch.equal(pools[0][0], pools[1][0]) and torch.equal(pools[0][1], pools[1][1])
+        peers.raise_errors()
+        peers.close()
+    finally:
+        if own_group:
+            dist.destroy_process_group()
+
+
 # ---------------------------------------------------------------- together
 
 
