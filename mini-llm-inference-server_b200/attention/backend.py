@@ -123,6 +123,9 @@ class B200Backend(AttentionBackend):
         pool_block = BLOCK_SIZE if fp4 else k_cache.shape[1]
         if pool_block != meta.block_size:
             raise ValueError(f"pool block size {pool_block} != metadata block size {meta.block_size}")
+        if fp4 and (q.dtype is torch.float32 or q.shape[1] > 8 * pool_kv_heads(k_cache)):  # before anything is written
+            raise ValueError(f"4-bit pools: queries must be float16 or bfloat16 with at most 8 heads per KV head, got "
+                             f"{q.dtype}, {q.shape[1]} heads on {pool_kv_heads(k_cache)}")
         err = self._error_word(q.device) if self.check_errors else None
         plan = self.plan(meta, q.shape[1], pool_kv_heads(k_cache), q.device, k_cache.dtype)
         append = None

@@ -20,7 +20,8 @@
 // most pages need one vote instead of the maximum over the lanes and no rescaling of O; only pages on an edge (the
 // row's end, a causal limit) test their keys.
 // What bounds it: bytes for long rows, the conversions' instructions and a CTA's start and end for short ones.  32 + 8
-// heads of 128 dims: 16 rows of 131072 tokens 386 us, 5.9 TB/s (90% of a copy); 64 rows of
+// heads of 128 dims: 16 rows of 131072 tokens 386 us, 5.9 TB/s (90% of a copy; repeated for seconds 450, the SM clock
+// then lowered from 1965 to 1690 MHz by the power limit, so it is the instructions that count there too); 64 rows of
 // 512..4096 tokens 40.5 us, 3.9 TB/s, issue slots 60% busy (16-bit pools 97 us); one row of 32001 tokens 17 us.
 // 4 warps a CTA and 4 CTAs an SM: 5 or 6 CTAs spill, and 2 or 8 warps a CTA were slower.
 #include <climits>

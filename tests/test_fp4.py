@@ -98,6 +98,19 @@ def test_entry_points_refuse_tensors_of_the_cpu(mlb):
         mlb.paged_attention_fp4(x.bfloat16(), p, p, i32, i32[0], i32[0], plan)
 
 
+def test_backend_refuses_queries_before_it_writes(mlb):
+    backend = mlb.get_backend("b200")
+    meta = mlb.AttentionMetadata.build([mlb.SeqStep(0, 2, [1])], 16, "cpu")
+    pools = [torch.full((3, 2, 17, 64), 7, dtype=torch.uint8) for _ in range(2)]
+    k = torch.zeros(2, 2, 128, dtype=torch.bfloat16)
+    for q in (torch.zeros(2, 8, 128), torch.zeros(2, 18, 128, dtype=torch.bfloat16)):
+        with pytest.raises(ValueError, match="at most 8 heads per KV head"):
+            backend.forward(q, k.to(q.dtype), k.to(q.dtype), *pools, meta)
+    with pytest.raises(ValueError, match="block size"):
+        backend.forward(k, k, k, *pools, mlb.AttentionMetadata.build([mlb.SeqStep(0, 2, [1])], 32, "cpu"))
+    assert all((p == 7).all() for p in pools)
+
+
 def test_rotary_table_refusals_and_values(mlb):
     for rows, rot in ((0, 64), (8, 0), (8, 24), (-1, 16)):
         with pytest.raises(ValueError, match="rotary_table"):
