@@ -533,10 +533,11 @@ def attention_partials_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
         out, o0, o1 = None, 0, 0
     else:
         if out is None:
-            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            out, o0, o1 = torch.empty_like(q, memory_format=torch.contiguous_format), h * dh, dh
         elif out.shape != shape or out.dtype != q.dtype or out.get_device() != dev or (n and out.stride(2) != 1):
             raise ValueError(f"{what}: out must match q")
-        o0, o1, _ = out.stride()
+        else:
+            o0, o1, _ = out.stride()
     if n == 0 or plan.num_units + plan.num_shared_units == 0:
         return out
     po = plse = None
@@ -605,11 +606,12 @@ class Rotary:
 
 
 def _check_rope(what: str, q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor,
-                q_weight: torch.Tensor | None, k_weight: torch.Tensor | None) -> int:
+                q_weight: torch.Tensor | None, k_weight: torch.Tensor | None) -> tuple:
+    """(dtype code, q's shape, KV heads, device ordinal, q's strides, k's strides)"""
     qs, dt, dev, code = q.shape, q.dtype, q.get_device(), DTYPE_CODE.get(q.dtype)
-    ks = k.shape
+    ks, q_st, k_st = k.shape, q.stride(), k.stride()
     if (len(qs) == 3 and len(ks) == 3 and qs[0] == ks[0] and qs[2] == ks[2] and qs[2] in (64, 128, 256)
-            and q.stride()[2] == 1 and k.stride()[2] == 1 and code is not None and k.dtype is dt and dev >= 0
+            and q_st[2] == 1 and k_st[2] == 1 and code is not None and k.dtype is dt and dev >= 0
             and k.get_device() == dev and positions.dtype is torch.long and positions.shape == qs[:1]
             and positions.is_contiguous() and positions.get_device() == dev and cos_sin.dtype is torch.float32
             and cos_sin.dim() == 2 and cos_sin.is_contiguous() and cos_sin.get_device() == dev
@@ -617,7 +619,7 @@ def _check_rope(what: str, q: torch.Tensor, k: torch.Tensor, positions: torch.Te
                                       and q_weight.get_device() == dev))
             and (k_weight is None or (k_weight.shape == qs[2:] and k_weight.dtype is dt and k_weight.is_contiguous()
                                       and k_weight.get_device() == dev))):
-        return code
+        return code, qs, ks[1], dev, q_st, k_st
     if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
         raise ValueError(f"{what}: q must be [N, H, Dh] and k [N, Hkv, Dh], got {tuple(q.shape)}, {tuple(k.shape)}")
     dh = q.shape[2]
@@ -634,7 +636,7 @@ def _check_rope(what: str, q: torch.Tensor, k: torch.Tensor, positions: torch.Te
     for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
         if w is not None and (w.shape != (dh,) or w.dtype != q.dtype or w.device != q.device or not w.is_contiguous()):
             raise ValueError(f"{what}: {name} must be a contiguous [{dh}] tensor of q's dtype on {q.device}")
-    return _code(q, what)
+    return _code(q, what), qs, ks[1], dev, q_st, k_st
 
 
 def _check_row_out(what: str, out: torch.Tensor, x: torch.Tensor) -> None:
@@ -660,19 +662,19 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, cos_
     `rotary_table`, its rot_dim at most Dh (the dims behind it are not rotated).  out = (q_out, k_out) may be
     (q, k), else memory that overlaps neither.  Rows whose position is outside the table are left unwritten."""
     what = "qk_norm_rope"
-    code = _check_rope(what, q, k, positions, cos_sin, q_weight, k_weight)
-    n, h, dh = q.shape
+    code, (n, h, dh), hkv, dev, qs, ks = _check_rope(what, q, k, positions, cos_sin, q_weight, k_weight)
     if out is None:
         qo = torch.empty_like(q, memory_format=torch.contiguous_format)
         ko = torch.empty_like(k, memory_format=torch.contiguous_format)
+        qos, kos = (h * dh, dh), (hkv * dh, dh)
     else:
         qo, ko = out
         _check_row_out(what, qo, q)
         _check_row_out(what, ko, k)
-    qs, ks, qos, kos = q.stride(), k.stride(), qo.stride(), ko.stride()
+        qos, kos = qo.stride(), ko.stride()
     rows, rot = cos_sin.shape
-    _launch(_lib.QK_NORM_ROPE, what, q.get_device(), q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], code,
-            n, h, k.shape[1], dh, positions.data_ptr(), cos_sin.data_ptr(), rows, rot, _adr(q_weight), _adr(k_weight),
+    _launch(_lib.QK_NORM_ROPE, what, dev, q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], code,
+            n, h, hkv, dh, positions.data_ptr(), cos_sin.data_ptr(), rows, rot, _adr(q_weight), _adr(k_weight),
             eps, qo.data_ptr(), qos[0], qos[1], ko.data_ptr(), kos[0], kos[1], _adr(err))
     return qo, ko
 
@@ -686,22 +688,21 @@ def qk_norm_rope_append_fp4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, p
     bit-identical to the two calls'.  cos_sin must rotate the whole head (rot_dim == Dh)."""
     what = "qk_norm_rope_append_fp4"
     nb, hkv, dh = _check_fp4_pools(k_cache, v_cache, what)
-    code = _check_rope(what, q, k, positions, cos_sin, q_weight, k_weight)
-    n, h, _ = q.shape
-    dev, ks, vs = q.get_device(), k.stride(), v.stride()
-    if not (k.shape[1] == hkv and k.shape[2] == dh and v.shape == k.shape and vs[2] == 1 and v.dtype is k.dtype
+    code, (n, h, q_dh), k_heads, dev, qs, ks = _check_rope(what, q, k, positions, cos_sin, q_weight, k_weight)
+    vs = v.stride()
+    if not (k_heads == hkv and q_dh == dh and v.shape == (n, hkv, dh) and vs[2] == 1 and v.dtype is k.dtype
             and v.get_device() == dev and k_cache.get_device() == dev and slot_mapping.dtype is torch.long
-            and slot_mapping.shape == q.shape[:1] and slot_mapping.is_contiguous() and slot_mapping.get_device() == dev):
+            and slot_mapping.shape == (n,) and slot_mapping.is_contiguous() and slot_mapping.get_device() == dev):
         _check_rows(k, hkv, dh, f"{what} k")
         _check_rows(v, hkv, dh, f"{what} v")
         if v.shape[0] != n or v.dtype != k.dtype or v.device != k.device or k_cache.device != k.device:
             raise ValueError(f"{what}: q, k, v and the pools must agree in rows, dtype and device")
         _check_index(slot_mapping, n, q.device, what, "slot_mapping")
     if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        out, os = torch.empty_like(q, memory_format=torch.contiguous_format), (h * dh, dh)
     else:
         _check_row_out(what, out, q)
-    qs, os = q.stride(), out.stride()
+        os = out.stride()
     rows, rot = cos_sin.shape
     _launch(_lib.QK_NORM_ROPE_APPEND_FP4, what, dev, q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1],
             v.data_ptr(), vs[0], vs[1], code, n, h, hkv, dh, positions.data_ptr(), cos_sin.data_ptr(), rows, rot,
