@@ -89,7 +89,13 @@ __device__ __forceinline__ void fp4_reciprocal(float scale, float& hi, float& lo
   hi = scale > 0.f ? __uint_as_float(__float_as_uint(r) - 1u) : 0.f;
   lo = scale > 0.f ? fmaf(-hi, scale, 1.f) * hi : 0.f;
 }
-__device__ __forceinline__ float fp4_quotient_16(float x, float hi, float lo) { return fmaf(x, hi, x * lo); }
+// x: of at most 11 significant bits; two quotients by packed operations.
+__device__ __forceinline__ void fp4_quotients_16(float& x0, float& x1, float hi, float lo) {
+  asm("{\n.reg .b64 x, h, l;\nmov.b64 x, {%0, %1};\nmov.b64 h, {%2, %2};\nmov.b64 l, {%3, %3};\n"
+      "mul.rn.f32x2 l, x, l;\nfma.rn.f32x2 x, x, h, l;\nmov.b64 {%0, %1}, x;\n}\n"
+      : "+f"(x0), "+f"(x1)
+      : "f"(hi), "f"(lo));
+}
 
 // The same for fp32 x, whose quotients can round onto a border that they only lie next to: an inexact quotient is made
 // odd in the direction of its remainder.

@@ -184,9 +184,9 @@ __device__ __forceinline__ void quant_store(const SlotRow<DH>& at, int c, const 
     fp4_reciprocal(fp4_scale_value(ba), ha, la);
     fp4_reciprocal(fp4_scale_value(bb), hb, lb);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      a[i] = fp4_quotient_16(a[i], ha, la);
-      b[i] = fp4_quotient_16(b[i], hb, lb);
+    for (int i = 0; i < 8; i += 2) {
+      fp4_quotients_16(a[i], a[i + 1], ha, la);
+      fp4_quotients_16(b[i], b[i + 1], hb, lb);
     }
     if (live) store_codes<DH>(at, c, fp4_pack8(a), fp4_pack8(b), ba, bb);
   }
