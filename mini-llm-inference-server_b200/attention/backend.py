@@ -118,7 +118,7 @@ class B200Backend(AttentionBackend):
         in every rank's gathered buffer of that slot (the reduction carries the all-gather: as flagged
         packets, or plain stores followed by the peers' barrier, as the PeerOutputs was built).
         rotary (optional, `ops.Rotary`): q and k come from the projection; norm and rotate them at
-        meta.positions first."""
+        meta.positions first.  Its table needs a row for every position of the step's new tokens."""
         fp4 = is_fp4(k_cache)
         pool_block = BLOCK_SIZE if fp4 else k_cache.shape[1]
         if pool_block != meta.block_size:
@@ -129,6 +129,9 @@ class B200Backend(AttentionBackend):
         err = self._error_word(q.device) if self.check_errors else None
         plan = self.plan(meta, q.shape[1], pool_kv_heads(k_cache), q.device, k_cache.dtype)
         append = None
+        if rotary is not None and plan.last_position >= rotary.cos_sin.shape[0]:  # such keys would hold no values
+            raise ValueError(f"rotary: position {plan.last_position} of a new token, the table has "
+                             f"{rotary.cos_sin.shape[0]} rows")
         if rotary is not None and not (fp4 and rotary.cos_sin.shape[1] == q.shape[2]):
             q, k = qk_norm_rope(q, k, meta.positions, rotary.cos_sin, rotary.q_weight, rotary.k_weight, rotary.eps,
                                 err=err)

@@ -118,6 +118,7 @@ class AttentionPlan:
     max_pieces: int = 0  # the most pieces of one token
     num_seqs: int = 0
     max_blocks: int = 0  # width of the block tables it was planned for
+    last_position: int = -1  # the largest position of a new token
 
 
 def _i32(a) -> np.ndarray:
@@ -176,7 +177,8 @@ def plan_attention(qo_indptr: list[int], seq_lens: list[int], max_blocks: int, n
                          max(1, 8 // (num_heads // num_kv_heads)), num_heads, num_kv_heads, n_tok,
                          units[:u].copy(), shared[:sh].copy(), members[:m].copy(), rows[:n_tok].copy(),
                          chunks[:n_tok].copy(), bool(sh and ((shared[:sh, 6] & 0xFF) == 1).any()),
-                         int(chunks[:n_tok].max()) if n_tok else 0, s, max_blocks)
+                         int(chunks[:n_tok].max()) if n_tok else 0, s, max_blocks,
+                         int(lens[qo[1:] > qo[:-1]].max()) - 1 if n_tok else -1)
 
 
 class Workspace:
@@ -660,7 +662,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, cos_
     one launch (mlb_qk_norm_rope): q [N, H, Dh], k [N, Hkv, Dh] -> the same shapes and dtype, computed in fp32.
     q and k may be views of a fused projection.  positions int64 [N] (AttentionMetadata.positions); cos_sin from
     `rotary_table`, its rot_dim at most Dh (the dims behind it are not rotated).  out = (q_out, k_out) may be
-    (q, k), else memory that overlaps neither.  Rows whose position is outside the table are left unwritten."""
+    (q, k), else memory that overlaps neither.  Rows whose position is outside the table are left unwritten (and
+    flagged in err): without `out` they hold no values, and must not be appended or attended."""
     what = "qk_norm_rope"
     code, (n, h, dh), hkv, dev, qs, ks = _check_rope(what, q, k, positions, cos_sin, q_weight, k_weight)
     if out is None:

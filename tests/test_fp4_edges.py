@@ -1,0 +1,28 @@
+"""Calls around the 4-bit cache that are refused, or decided on the host, where their first tests did not look."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+
+@pytest.mark.parametrize("rot", [64, 32, 0])
+@pytest.mark.parametrize("fp4", [True, False])
+def test_backend_refuses_positions_behind_the_rotation_table(mlb, fp4, rot):
+    """A key at such a position has no rotation: nothing may reach the cache, whichever launch would have made it."""
+    shape, dtype = ((4, 2, 17, 32), torch.uint8) if fp4 else ((4, 16, 2, 64), torch.bfloat16)
+    pools = [torch.full(shape, 7, dtype=dtype) for _ in range(2)]
+    meta = mlb.AttentionMetadata.build([mlb.SeqStep(0, 2, [1]), mlb.SeqStep(19, 1, [0, 2])], 16, "cpu")
+    q, k = torch.zeros(3, 8, 64, dtype=torch.bfloat16), torch.zeros(3, 2, 64, dtype=torch.bfloat16)
+    backend = mlb.get_backend("b200")
+    with pytest.raises(ValueError, match="position 19 .* 19 rows"):
+        backend.forward(q, k, k, *pools, meta, rotary=mlb.Rotary(torch.zeros(19, rot)))
+    assert all((p == 7).all() for p in pools)
+    with pytest.raises(ValueError, match="CUDA"):  # the last position that has a row: on to the entry points' own checks
+        backend.forward(q, k, k, *pools, meta, rotary=mlb.Rotary(torch.zeros(20, rot)))
+
+
+def test_plan_knows_the_last_position_of_a_new_token(mlb):
+    lens, width = [40, 900, 7], 57
+    for qo, last in (([0, 3, 3, 4], 39), ([0, 0, 1, 1], 899), ([0, 0, 0, 0], -1)):  # rows without new tokens do not count
+        assert mlb.plan_attention(qo, lens, width, 8, 2, "cpu").last_position == last
