@@ -451,7 +451,7 @@ MLB_API int mlb_qk_norm_rope_append_fp4(const void* q, int64_t q_stride_tok, int
 /*
  * mlb_paged_attention over 4-bit pools: q and out are fp16 or bf16, the plan is mlb_plan_attention's (units,
  * shared units and query tiles alike), partial rows are completed by mlb_splitk_reduce.  head_dim 64 / 128 / 256,
- * at most 8 query heads per KV head, scale positive.  Stored values enter the products exactly; P is rounded to
+ * at most 8 query heads per KV head, scale positive and finite times log2(e).  Stored values enter the products exactly; P is rounded to
  * fp16, sums are fp32.
  */
 MLB_API int mlb_paged_attention_fp4(const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k_cache,

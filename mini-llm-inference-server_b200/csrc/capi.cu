@@ -1040,7 +1040,8 @@ int mlb_paged_attention_fp4(const void* q, int64_t q_stride_tok, int64_t q_strid
     return fail(MLB_EINVAL, "%s: num_heads %d not a multiple of num_kv_heads %d", what, num_heads, num_kv_heads);
   if (num_heads / num_kv_heads > 8)
     return fail(MLB_EUNSUPPORTED, "%s: %d query heads per KV head (at most 8)", what, num_heads / num_kv_heads);
-  if (!(scale > 0.f) || !(scale <= 3.4028235e38f)) return fail(MLB_EINVAL, "%s: scale must be positive and finite", what);
+  if (!(scale > 0.f) || !std::isfinite(scale * mlb::kLog2e))
+    return fail(MLB_EINVAL, "%s: scale must be positive, and finite times log2(e)", what);
   if (num_units < 0 || num_shared_units < 0 || num_seqs < 0 || num_blocks <= 0 || num_partial_rows < 0)
     return fail(MLB_EINVAL, "%s: bad sizes", what);
   if (num_units == 0 && num_shared_units == 0) return MLB_OK;

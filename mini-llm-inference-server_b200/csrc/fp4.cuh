@@ -114,5 +114,10 @@ __device__ __forceinline__ void fp4_query_scale(float mx, float& up, float& down
   down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
   up = __uint_as_float(static_cast<uint32_t>(e) << 23);
 }
+// The softmax scale of such a row: a positive finite number.  At zero a masked score (-inf) would become NaN; at or
+// below the smallest normal number every weight is 1 (sums of products stay below 2^39, so exponents below 2^-87).
+__device__ __forceinline__ float fp4_softmax_scale(float sl2, float up) {
+  return fminf(fmaxf(sl2 * up, 1.17549435e-38f), 3.4028235e38f);
+}
 
 }  // namespace mlb

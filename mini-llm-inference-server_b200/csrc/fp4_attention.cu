@@ -112,7 +112,7 @@ struct Columns {
 template <int DT, int DH>
 __device__ __forceinline__ void load_queries(Columns<DH>& c, const AttnArgs& a, const uint16_t* qrow, bool live, int lane) {
   constexpr int N = DH / 4;
-  float f = 1.f;
+  float s = a.sl2;
   if (live) {
     const uint16_t* src = qrow + (lane & 3) * N;
     uint32_t w[N / 2];
@@ -142,15 +142,15 @@ __device__ __forceinline__ void load_queries(Columns<DH>& c, const AttnArgs& a, 
     }
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-    float down;
-    fp4_query_scale(mx, f, down);
+    float up, down;
+    fp4_query_scale(mx, up, down);
+    s = fp4_softmax_scale(s, up);
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) {
       const uint32_t w = c.qb[i >> 1][i & 1];
       c.qb[i >> 1][i & 1] = pack2<MLB_F16>(__uint_as_float(w << 16) * down, __uint_as_float(w & 0xffff0000u) * down);
     }
   }
-  const float s = a.sl2 * f;
   c.sl2[0] = __shfl_sync(0xffffffffu, s, (lane & 3) * 8);
   c.sl2[1] = __shfl_sync(0xffffffffu, s, (lane & 3) * 8 + 4);
 }

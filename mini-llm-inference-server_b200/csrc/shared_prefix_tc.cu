@@ -549,7 +549,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           mx = fmaxf(mx, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u))));
         float up, down;
         fp4_query_scale(mx, up, down);
-        sl2 *= up;
+        sl2 = fp4_softmax_scale(sl2, up);
 #pragma unroll
         for (int ch = 0; ch < CH; ++ch) {
           uint32_t h[4];

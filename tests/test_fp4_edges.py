@@ -26,3 +26,17 @@ def test_plan_knows_the_last_position_of_a_new_token(mlb):
     lens, width = [40, 900, 7], 57
     for qo, last in (([0, 3, 3, 4], 39), ([0, 0, 1, 1], 899), ([0, 0, 0, 0], -1)):  # rows without new tokens do not count
         assert mlb.plan_attention(qo, lens, width, 8, 2, "cpu").last_position == last
+
+
+def test_attention_refuses_a_scale_that_overflows(mlb):
+    """scale * log2(e) is what the kernels multiply by."""
+    L = mlb.ops._lib
+
+    def call(scale):
+        f = 1 << 20  # a pointer that is never followed
+        return L.lib().mlb_paged_attention_fp4(f, 512, 64, f, f, 2, 4, 8, 2, 64, scale, f, 1, f, f, 1, f, 0, None, 0, None,
+                                               None, None, 0, f, 512, 64, None, None, None)
+
+    assert call(2.3e38) == L.MLB_OK  # no units: nothing to do
+    for scale in (2.5e38, 3.4e38, -2.5e38):
+        assert call(scale) == L.MLB_EINVAL and "scale" in L.last_error()
