@@ -107,6 +107,14 @@ __device__ __forceinline__ float fp4_quotient_32(float x, float scale, float hi,
   return __uint_as_float(u);
 }
 
+// P in fp16.  A row's probabilities are 2^(score - m) with m between kFp4Lift and kFp4Lift + kFp4Rise below the largest
+// score so far: at most 2^14, and normal fp16 numbers (2^-11 relative) down to 2^-24 of the largest one.  Below that they
+// lie on a grid of 2^-34 of it (with m at the largest score itself the grid is 2^-24, and the weight of 40000 keys that
+// e^18 divides, a thousandth of the row, was lost).  m moves when a score rises by more than kFp4Rise above the one it was
+// taken from, which after the first pages is rare; sums and O are fp32 and carry the lift until O is divided by the sum.
+constexpr float kFp4Lift = 10.f;
+constexpr float kFp4Rise = 4.f;
+
 // bf16 query rows enter fp16 products divided by the power of two of their largest element mx: down = 2^-e, up = 2^e,
 // with e kept where both are normal numbers.
 __device__ __forceinline__ void fp4_query_scale(float mx, float& up, float& down) {

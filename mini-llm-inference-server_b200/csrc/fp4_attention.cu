@@ -15,10 +15,10 @@
 // All products are fp16 x fp16 with fp32 sums, also for bf16 queries: a query row is first divided by the power of
 // two of its largest element (exact: bf16 has 8 significant bits, fp16 11; elements 2^-14 below the row's largest
 // and less lose bits that are 2^-25 of it) and the exponent goes into the row's softmax scale.
-// P is rounded to fp16 (2^-11 relative at most), 8 times finer than a bf16 output.
-// The running maximum moves only when a page's scores exceed it by more than 8 (a factor 256, far inside fp16), so
-// most pages need one vote instead of the maximum over the lanes and no rescaling of O; only pages on an edge (the
-// row's end, a causal limit) test their keys.
+// P is rounded to fp16: 2^-11 relative, 8 times finer than a bf16 output, for weights down to 2^-24 of the largest, on a
+// grid of 2^-34 of it below (kFp4Lift).  The running maximum moves only when a page's scores exceed the one it was taken
+// from by more than 4 (kFp4Rise), so most pages need one vote instead of the maximum over the lanes and no rescaling of
+// O; only pages on an edge (the row's end, a causal limit) test their keys.
 // What bounds it: bytes for long rows, the conversions' instructions and a CTA's start and end for short ones.  32 + 8
 // heads of 128 dims: 16 rows of 131072 tokens 386 us, 5.9 TB/s (90% of a copy; repeated for seconds 450, the SM clock
 // then lowered from 1965 to 1690 MHz by the power limit, so it is the instructions that count there too); 64 rows of
@@ -99,11 +99,11 @@ struct Columns {
   uint32_t qb[DH / 16][2];
   float o[DH / 16][4];
   float sl2[2];  // softmax scale * log2(e) * the power of two taken out of the column's query
-  float nb[2];   // minus the maximum in use (exp2 domain), or kUnset
+  float nb[2];   // minus the exponent taken off every score (exp2 domain; the maximum in use less kFp4Lift), or kUnset
   float l[2];
   int lim[2];  // exclusive key limits
   int all;     // the smallest limit of the warp's live columns: pages below it are seen whole
-  // before a column has seen a key: any finite score lies above "the maximum", so the first page sets it
+  // before a column has seen a key: any finite score lies above it, so the first page sets it
   static constexpr float kUnset = 1e30f;
   __device__ __forceinline__ float m(int i) const { return nb[i] == kUnset ? kNegInf : -nb[i]; }
 };
@@ -278,7 +278,7 @@ __device__ __forceinline__ void attend_fp4_pages(Columns<DH>& c, uint32_t slot, 
                      (t0 + 9 < live ? 0xff000000u : 0u);
     }
   }
-  // scores relative to the maximum in use, exp2 domain
+  // scores less the columns' exponents, exp2 domain
   float y[2][4];
 #pragma unroll
   for (int h = 0; h < 2; ++h)
@@ -286,7 +286,7 @@ __device__ __forceinline__ void attend_fp4_pages(Columns<DH>& c, uint32_t slot, 
     for (int i = 0; i < 4; ++i) y[h][i] = fmaf(s[h][i], c.sl2[i & 1], c.nb[i & 1]);
   const float top = fmaxf(fmaxf(fmaxf(y[0][0], y[0][1]), fmaxf(y[0][2], y[0][3])),
                           fmaxf(fmaxf(y[1][0], y[1][1]), fmaxf(y[1][2], y[1][3])));
-  if (__any_sync(0xffffffffu, top > 8.f)) {
+  if (__any_sync(0xffffffffu, top > kFp4Lift + kFp4Rise)) {
     float mx[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -297,7 +297,7 @@ __device__ __forceinline__ void attend_fp4_pages(Columns<DH>& c, uint32_t slot, 
     float al[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const float m = c.m(i), mn = fmaxf(m, mx[i]);
+      const float m = c.m(i), mn = fmaxf(m, mx[i] - kFp4Lift);
       al[i] = m == kNegInf ? 0.f : fast_exp2(m - mn);
       c.l[i] *= al[i];
       c.nb[i] = mn == kNegInf ? c.kUnset : -mn;

@@ -28,9 +28,9 @@
 //   packed to 16 bits, goes back over the first 64 columns of the same S buffer; row sums in fp32.  The 128
 //   scores per thread need more than the 168 registers 384 threads get at launch: warps 0-3 give theirs up
 //   (setmaxnreg.dec to 56) and the softmax warps take them (setmaxnreg.inc to 224).  O is rescaled (TMEM load /
-//   scale / store) only when a row's max grows by more than 8 (a factor 256 of headroom keeps P and the
-//   sums finite), which after the first tiles is rare; the rescale first waits for the P . V products
-//   before it.  At the end (the "final" barrier, committed behind the last MMA) every column's normalised O
+//   scale / store) only when a row's max grows by more than 8 (4-bit pools 4, with P lifted by 2^10: fp4.cuh),
+//   which after the first tiles is rare and keeps P and the sums finite; the rescale first waits for the P . V
+//   products before it.  At the end (the "final" barrier, committed behind the last MMA) every column's normalised O
 //   row and log2-sum-exp go to its split-K partial row, merged by the reduction (an unsplit query tile
 //   stores its final rows).
 // TMEM columns, paired: S_A [0,128), S_B [128,256), O_A [256, 256 + Dh), O_B [256 + Dh, 256 + 2 Dh);
@@ -258,6 +258,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   constexpr uint32_t kIdescS = f16_idesc(kFmt, false, kTcRows, kTcTileTokens);
   constexpr uint32_t kIdescO = f16_idesc(kFmt, true, kTcRows, DH);
   constexpr float kNegInfF = -__builtin_huge_valf();
+  // how far the exponent taken off a row's scores lies below its maximum, and how far that may rise before it is moved
+  constexpr float kLift = FP4 ? kFp4Lift : 0.f, kRise = FP4 ? kFp4Rise : 8.f;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBarOffset);
@@ -667,9 +669,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
       }
       const float mx = mraw * sl2;  // the scale is positive: max commutes with it
-      const bool need = mx > m_used + 8.f;
+      const bool need = mx > m_used + (kLift + kRise);
       if (__any_sync(0xffffffffu, need)) {
-        const float m_new = need ? fmaxf(m_used, mx) : m_used;
+        const float m_new = need ? fmaxf(m_used, mx - kLift) : m_used;
         if (j > 0) {  // paired: P_x(j-1) . V has completed (s_full[x] of this tile was committed after it)
           if (!two && !wait_warp(o_done, (j - 1) & 1)) {  // single: wait for it
             ok = false;

@@ -1,6 +1,9 @@
-"""The 4-bit operators where their first tests did not look: scales next to nothing."""
+"""The 4-bit operators where their first tests did not look: scales next to nothing, weights far below the
+largest."""
 
 from __future__ import annotations
+
+import math
 
 import pytest
 import torch
@@ -8,6 +11,37 @@ import torch
 from test_fp4_gpu import Step
 
 pytestmark = pytest.mark.gpu
+
+
+class Rows:
+    """Rows of given keys, values and queries: key and value of position p are k[p], v[p] for every row and head, and
+    have to be values that the 4-bit format holds."""
+
+    def __init__(self, mlb, cuda, h, hkv, steps, k, v, q, dtype, how="plain"):
+        dh = k.shape[1]
+        need = [-(-(c + n) // 16) for c, n in steps]
+        ids = torch.randperm(sum(need), generator=torch.Generator().manual_seed(1)).tolist()
+        self.seqs = [(c, n, [ids.pop() for _ in range(m)]) for (c, n), m in zip(steps, need)]
+        self.pools = [torch.full((sum(need), hkv, 17, dh // 2), 0xFF, dtype=torch.uint8, device=cuda) for _ in range(2)]
+        for c, n, blk in self.seqs:
+            p = torch.arange(c + n)
+            slots = (torch.tensor(blk)[p // 16] * 16 + p % 16).to(cuda)
+            rows = [x[:c + n, None].expand(-1, hkv, -1).to(dtype).to(cuda) for x in (k, v)]
+            mlb.kv_append_fp4(*self.pools, slots, *rows)
+            for got, want in zip(mlb.kv_read_fp4(*self.pools, slots, dtype), rows):
+                assert torch.equal(got, want)
+        n = sum(x for _, x in steps)
+        wide = torch.zeros(n, h, dh + 3, dtype=dtype, device=cuda)  # "odd": rows off 16-byte alignment
+        self.q = q.to(dtype).to(cuda).expand(n, h, dh).contiguous() if how == "plain" else wide[:, :, 1:dh + 1].copy_(q)
+        self.meta = mlb.AttentionMetadata.build([mlb.SeqStep(*s) for s in self.seqs], 16, cuda)
+        self.heads, self.seen = (h, hkv), [c + i + 1 for c, n in steps for i in range(n)]  # keys that each token sees
+
+    def run(self, mlb, cuda, tables=True, pages=0, **kw):
+        m = self.meta
+        plan = mlb.plan_attention(m.query_start_loc, m.seq_lens, m.block_tables_i32.shape[1], *self.heads, cuda,
+                                  pages_per_unit=pages, pool_dtype=torch.uint8,
+                                  block_tables_host=m.block_tables_host if tables else None)
+        return mlb.paged_attention_fp4(self.q, *self.pools, m.block_tables_i32, m.seq_lens_i32, m.qo_indptr, plan, **kw)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
@@ -20,3 +54,24 @@ def test_zero_queries_under_a_tiny_scale(mlb, cuda, dtype, scale):
         st.q_dev.copy_(st.q)
         for tables, pages in ((True, 0), (False, 0), (False, 2)):
             st.check(st.run(mlb, cuda, tables, pages, scale=scale), scale=scale)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tables,how", [(True, "plain"), (True, "odd"), (False, "plain")])
+def test_a_long_tail_keeps_its_weight(mlb, cuda, dtype, tables, how):
+    """One key weighs e^18 times each of the 40000 others; its value is 0, theirs 6, so what comes out is the others'
+    weight.  A weight is 2^-25.97 of the largest: rounded on a grid of 2^-34 (fp16 at 2^10 times the weight) it is off
+    by at most 2^-35 / 2^-25.97 = 2^-9.03; fp32 sums of 2500 pages and the merge, 2^-23 an addition, twice: 2^-10.7;
+    the exponent's argument, 26 with 2 roundings of 2^-24, times ln 2 and twice: 2^-18; then the output's rounding."""
+    length, dh = 40040, 64
+    k, v = torch.zeros(length, dh), torch.full((length, dh), 6.0)
+    k[0, 0], v[0] = 18.0, 0.0
+    q = torch.zeros(dh)
+    q[0] = 1.0
+    st = Rows(mlb, cuda, 4, 1, [(40000, 1), (40000, 20)], k, v, q, dtype, how)
+    rel = 2.0**-9.03 + 2.0**-10.7 + 2.0**-18 + torch.finfo(dtype).eps / 2
+    for pages in (1 << 20, 0):
+        got = st.run(mlb, cuda, tables, pages, scale=1.0).cpu().double()
+        tail = (torch.tensor(st.seen, dtype=torch.float64) - 1) * math.exp(-18)
+        want = (6 * tail / (1 + tail))[:, None, None]
+        assert ((got - want).abs() <= rel * want).all(), ((got - want).abs() / want).max().item()
