@@ -115,10 +115,13 @@ __device__ __forceinline__ float fp4_quotient_32(float x, float scale, float hi,
 constexpr float kFp4Lift = 10.f;
 constexpr float kFp4Rise = 4.f;
 
-// bf16 query rows enter fp16 products divided by the power of two of their largest element mx: down = 2^-e, up = 2^e,
-// with e kept where both are normal numbers.
+// bf16 query rows enter fp16 products divided by a power of two that brings their largest element mx to [2^14, 2^15):
+// down = 2^-e, up = 2^e, both normal numbers (a row below 2^-112 stays below 2^14).  A bf16 element keeps its 8 bits
+// down to 2^-31 of the row's largest (the lowest of them then weighs 2^-24, the step of fp16's subnormal numbers), and
+// smaller ones lie on a grid of 2^-38 of it: finer than what an fp32 sum with the row's largest would leave of them.
+// Sums stay far inside fp32: 2^15 x 61440 x 256 products is below 2^39.
 __device__ __forceinline__ void fp4_query_scale(float mx, float& up, float& down) {
-  const int e = max(1, min(static_cast<int>(__float_as_uint(mx) >> 23), 253));  // biased exponent
+  const int e = max(1, static_cast<int>(__float_as_uint(mx) >> 23) - 14);  // biased exponent, at most 241
   down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
   up = __uint_as_float(static_cast<uint32_t>(e) << 23);
 }

@@ -12,9 +12,9 @@
 //   O^T[Dh x 8] += V^T . P^T: lane g takes dims [g Dh / 8, (g + 1) Dh / 8) of tokens 2t, 2t + 1, 2t + 8, 2t + 9; a
 //   exchange of nibbles between two tokens' words makes bytes of one dim and two tokens, so that a cvt gives the
 //   (token, token + 1) pairs of the fragment, which are then multiplied by the tokens' pair of scales.
-// All products are fp16 x fp16 with fp32 sums, also for bf16 queries: a query row is first divided by the power of
-// two of its largest element (exact: bf16 has 8 significant bits, fp16 11; elements 2^-14 below the row's largest
-// and less lose bits that are 2^-25 of it) and the exponent goes into the row's softmax scale.
+// All products are fp16 x fp16 with fp32 sums, also for bf16 queries: a query row is first divided by a power of two
+// that brings its largest element to [2^14, 2^15) (exact: bf16 has 8 significant bits, fp16 11; only elements 2^-31
+// below the row's largest and less lose bits) and the exponent goes into the row's softmax scale (fp4.cuh).
 // P is rounded to fp16: 2^-11 relative, 8 times finer than a bf16 output, for weights down to 2^-24 of the largest, on a
 // grid of 2^-34 of it below (kFp4Lift).  The running maximum moves only when a page's scores exceed the one it was taken
 // from by more than 4 (kFp4Rise), so most pages need one vote instead of the maximum over the lanes and no rescaling of

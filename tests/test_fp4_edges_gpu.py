@@ -1,5 +1,5 @@
 """The 4-bit operators where their first tests did not look: scales next to nothing, weights far below the
-largest."""
+largest, query elements far below the row's."""
 
 from __future__ import annotations
 
@@ -14,8 +14,8 @@ pytestmark = pytest.mark.gpu
 
 
 class Rows:
-    """Rows of given keys, values and queries: key and value of position p are k[p], v[p] for every row and head, and
-    have to be values that the 4-bit format holds."""
+    """Rows of given keys, values and queries: key and value of position p are k[p], v[p] for every row and head.  The
+    keys have to be values that the 4-bit format holds; `held` are the values that the cache has of v, by position."""
 
     def __init__(self, mlb, cuda, h, hkv, steps, k, v, q, dtype, how="plain"):
         dh = k.shape[1]
@@ -28,8 +28,9 @@ class Rows:
             slots = (torch.tensor(blk)[p // 16] * 16 + p % 16).to(cuda)
             rows = [x[:c + n, None].expand(-1, hkv, -1).to(dtype).to(cuda) for x in (k, v)]
             mlb.kv_append_fp4(*self.pools, slots, *rows)
-            for got, want in zip(mlb.kv_read_fp4(*self.pools, slots, dtype), rows):
-                assert torch.equal(got, want)
+            keys, values = mlb.kv_read_fp4(*self.pools, slots, dtype)
+            assert torch.equal(keys, rows[0])
+            self.held = values[:, 0].cpu().double()
         n = sum(x for _, x in steps)
         wide = torch.zeros(n, h, dh + 3, dtype=dtype, device=cuda)  # "odd": rows off 16-byte alignment
         self.q = q.to(dtype).to(cuda).expand(n, h, dh).contiguous() if how == "plain" else wide[:, :, 1:dh + 1].copy_(q)
@@ -70,8 +71,25 @@ def test_a_long_tail_keeps_its_weight(mlb, cuda, dtype, tables, how):
     q[0] = 1.0
     st = Rows(mlb, cuda, 4, 1, [(40000, 1), (40000, 20)], k, v, q, dtype, how)
     rel = 2.0**-9.03 + 2.0**-10.7 + 2.0**-18 + torch.finfo(dtype).eps / 2
+    assert torch.equal(st.held, v[:len(st.held)].double())
     for pages in (1 << 20, 0):
         got = st.run(mlb, cuda, tables, pages, scale=1.0).cpu().double()
         tail = (torch.tensor(st.seen, dtype=torch.float64) - 1) * math.exp(-18)
         want = (6 * tail / (1 + tail))[:, None, None]
         assert ((got - want).abs() <= rel * want).all(), ((got - want).abs() / want).max().item()
+
+
+@pytest.mark.parametrize("tables,how", [(True, "plain"), (True, "odd"), (False, "plain")])
+def test_a_small_query_element_meets_a_large_key(mlb, cuda, tables, how):
+    """A bf16 query of 2048 and 1.5 * 2^-14, keys of 0 and 61440: the score is the small element's alone, 0.70.  Its one
+    product is exact, the exponent's argument has 2 roundings of 2^-24; a weight is rounded to 2^-11, twice."""
+    k, v = torch.zeros(120, 64), torch.zeros(120, 64)
+    k[::2, 1], v[::2] = 61440.0, 1.0
+    q = torch.zeros(64)
+    q[0], q[1] = 2048.0, 1.5 * 2.0**-14
+    st = Rows(mlb, cuda, 4, 1, [(50, 1), (100, 20)], k, v, q, torch.bfloat16, how)
+    got = st.run(mlb, cuda, tables).cpu().double()
+    seen = torch.tensor(st.seen, dtype=torch.float64)
+    top = torch.ceil(seen / 2) * math.exp(1.5 * 2.0**-14 * 61440 / 8)
+    want = (top / (top + torch.floor(seen / 2)))[:, None, None] * st.held[0]
+    assert ((got - want).abs() <= (2.0**-8 + 2.0**-10) * want).all(), ((got - want).abs() / want).max().item()
