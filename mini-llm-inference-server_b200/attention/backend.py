@@ -171,6 +171,11 @@ class B200Backend(AttentionBackend):
             self.raise_device_errors()
         return out
 
+    def release_scratch(self) -> None:
+        """Free the split-K scratch that larger steps have outgrown (`Workspace.release`).  No graph captured with this
+        backend before may be replayed after."""
+        self._workspace.release()
+
     # ------------------------------------------------------------------ device error word
     def _error_word(self, device: torch.device) -> torch.Tensor:
         if self._err is None or self._err.device != device:

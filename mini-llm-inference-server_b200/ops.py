@@ -181,32 +181,76 @@ def plan_attention(qo_indptr: list[int], seq_lens: list[int], max_blocks: int, n
                          int(lens[qo[1:] > qo[:-1]].max()) - 1 if n_tok else -1)
 
 
+class _Scratch:
+    """One pair of a workspace's buffers, and what has been done with it."""
+
+    __slots__ = ("o", "lse", "small", "captured", "streams")
+
+    def __init__(self, size_o: int, size_l: int, device: torch.device) -> None:
+        self.o, self.lse = (torch.empty(max(n, 1), dtype=torch.float32, device=device) for n in (size_o, size_l))
+        self.small = 4 * (self.o.numel() + self.lse.numel()) <= Workspace.SMALL_BYTES
+        self.captured = False  # handed out during a stream capture: a graph holds its address
+        self.streams: set[int] = set()  # streams that the allocator knows it is used on
+
+
 class Workspace:
-    """Split-K scratch (fp32 partial rows + their log-sum-exp), grown on demand and reused across calls.  What it
-    has outgrown stays allocated as long as the workspace (a captured graph may hold its address); it grows by half
-    at least, so that all of it stays below three times the largest."""
+    """Split-K scratch (fp32 partial rows + their log-sum-exp), grown on demand and reused across calls; one buffer of
+    each kind per device.  An outgrown one that was handed out during a stream capture stays allocated, since the graph
+    holds its address, until `release`; so does a small one.  What replaces those is larger by half at least, so that
+    all of them together stay below three times the largest.  Every other outgrown buffer goes back to the allocator
+    before its successor is made, which is no larger than asked for."""
+
+    SMALL_BYTES = 1 << 24  # a decode step's scratch: kept whatever held it, so that its calls need not look
 
     def __init__(self) -> None:
-        self._o: torch.Tensor | None = None
-        self._lse: torch.Tensor | None = None
-        self._held: list[tuple[torch.Tensor, torch.Tensor]] = []
+        self._pairs: dict[torch.device, list[_Scratch]] = {}  # outgrown ones that stay, then the one in use
 
     def get(self, rows: int, heads: int, dh: int, device: torch.device) -> tuple[torch.Tensor, torch.Tensor]:
         need_o, need_l = rows * heads * dh, rows * heads
-        if self._o is None or self._o.device != device or self._o.numel() < need_o or self._lse.numel() < need_l:
-            self._grow(need_o, need_l, device)
-        return self._o, self._lse
+        pairs = self._pairs.get(device)
+        if not pairs or pairs[-1].o.numel() < need_o or pairs[-1].lse.numel() < need_l:
+            pairs = self._grow(need_o, need_l, device)
+        p = pairs[-1]
+        if not p.small and not p.captured and device.type == "cuda":
+            if _capturing(device):
+                p.captured = True
+            elif _stream(device) not in p.streams:  # it is freed only when every stream is done with it
+                p.streams.add(_stream(device))
+                for t in (p.o, p.lse):
+                    t.record_stream(torch.cuda.current_stream(device))
+        return p.o, p.lse
 
-    def _grow(self, need_o: int, need_l: int, device: torch.device) -> None:
-        held = [(o, lse) for o, lse in self._held if o.device == device]
-        fits = [(o, lse) for o, lse in held if o.numel() >= need_o and lse.numel() >= need_l]
-        if not fits:
-            if held:
-                need_o, need_l = max(need_o, 3 * held[-1][0].numel() // 2), max(need_l, 3 * held[-1][1].numel() // 2)
-            fits = [(torch.empty(max(need_o, 1), dtype=torch.float32, device=device),
-                     torch.empty(max(need_l, 1), dtype=torch.float32, device=device))]
-            self._held += fits
-        self._o, self._lse = fits[-1]
+    def _grow(self, need_o: int, need_l: int, device: torch.device) -> list[_Scratch]:
+        pairs = self._pairs.setdefault(device, [])
+        if pairs:
+            last = pairs[-1]
+            size_o, size_l = last.o.numel(), last.lse.numel()
+            if last.small or last.captured:
+                size_o, size_l = 3 * size_o // 2, 3 * size_l // 2
+            else:
+                del pairs[-1]
+            del last
+            need_o, need_l = max(need_o, size_o), max(need_l, size_l)
+        pairs.append(_Scratch(need_o, need_l, device))
+        return pairs
+
+    def release(self) -> None:
+        """Free every outgrown buffer, once the GPU is done with them.  No graph that was captured with this workspace
+        before may be replayed after."""
+        for device, pairs in self._pairs.items():
+            if len(pairs) > 1 and device.type == "cuda":
+                torch.cuda.synchronize(device)
+            del pairs[:-1]
+            for p in pairs:
+                p.captured = False
+
+
+def _capturing(device: torch.device) -> bool:
+    """Whether torch's current stream on `device` is being captured into a graph."""
+    if torch.cuda.current_device() == device.index:
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(device):
+        return torch.cuda.is_current_stream_capturing()
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,

@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import weakref
+
 import pytest
 import torch
 
@@ -40,3 +42,26 @@ def test_attention_refuses_a_scale_that_overflows(mlb):
     assert call(2.3e38) == L.MLB_OK  # no units: nothing to do
     for scale in (2.5e38, 3.4e38, -2.5e38):
         assert call(scale) == L.MLB_EINVAL and "scale" in L.last_error()
+
+
+def test_workspace_gives_back_large_buffers_that_it_has_outgrown(mlb):
+    """Scratch of gigabytes (on the meta device: sizes without memory): one buffer at a time, no larger than asked."""
+    ws, dev = mlb.Workspace(), torch.device("meta")
+    first = [weakref.ref(t) for t in ws.get(1 << 17, 32, 128, dev)]
+    assert all(r() is not None for r in first)
+    o, lse = ws.get((1 << 17) + 1, 32, 128, dev)
+    assert o.numel() == ((1 << 17) + 1) * 32 * 128 and lse.numel() == ((1 << 17) + 1) * 32
+    assert all(r() is None for r in first)
+    assert ws.get(5, 32, 128, dev)[0] is o  # smaller asks share it
+    assert ws.get((1 << 16) + 2, 64, 64, dev)[0] is not o  # more row sums than it has
+    assert ws.get(1, 32, 128, torch.device("cpu"))[0].numel() == 32 * 128
+    assert ws.get((1 << 17) + 1, 32, 128, dev)[1].numel() == ((1 << 16) + 2) * 64
+
+
+def test_workspace_releases_what_it_keeps(mlb):
+    ws, dev = mlb.Workspace(), torch.device("cpu")
+    first = [weakref.ref(t) for t in ws.get(4, 2, 64, dev)]
+    last = ws.get(5, 2, 64, dev)
+    assert all(r() is not None for r in first)
+    ws.release()
+    assert all(r() is None for r in first) and ws.get(5, 2, 64, dev)[0] is last[0]

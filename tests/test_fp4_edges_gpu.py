@@ -4,6 +4,7 @@ largest, query elements far below the row's."""
 from __future__ import annotations
 
 import math
+import weakref
 
 import pytest
 import torch
@@ -93,3 +94,47 @@ def test_a_small_query_element_meets_a_large_key(mlb, cuda, tables, how):
     top = torch.ceil(seen / 2) * math.exp(1.5 * 2.0**-14 * 61440 / 8)
     want = (top / (top + torch.floor(seen / 2)))[:, None, None] * st.held[0]
     assert ((got - want).abs() <= (2.0**-8 + 2.0**-10) * want).all(), ((got - want).abs() / want).max().item()
+
+
+def test_workspace_keeps_only_what_a_graph_holds(mlb, cuda):
+    """Large buffers (above Workspace.SMALL_BYTES): dropped when outgrown, kept when a capture was given them."""
+    ws, dev = mlb.Workspace(), torch.zeros(1, device=cuda).device
+    rows = 1 << 13
+    first = [weakref.ref(t) for t in ws.get(rows, 8, 128, dev)]
+    assert 4 * first[0]().numel() > mlb.Workspace.SMALL_BYTES
+    second = [weakref.ref(t) for t in ws.get(rows + 1, 8, 128, dev)]
+    assert all(r() is None for r in first)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ws.get(rows, 8, 128, dev)[0].fill_(1.0)
+    third = [weakref.ref(t) for t in ws.get(rows + 2, 8, 128, dev)]
+    assert all(r() is not None for r in second) and third[0]().numel() == 3 * (rows + 1) * 8 * 128 // 2
+    g.replay()
+    torch.cuda.synchronize()
+    assert (second[0]() == 1).all()
+    del g
+    ws.get(2 * rows, 8, 128, dev)
+    assert all(r() is None for r in third)
+    ws.release()
+    assert all(r() is None for r in second)
+
+
+def test_an_outgrown_buffer_waits_for_the_stream_that_uses_it(mlb, cuda):
+    """Scratch of one stream, used on another and outgrown there: its memory is not given out before that stream is
+    done with it."""
+    ws, dev = mlb.Workspace(), torch.zeros(1, device=cuda).device
+    rows = 1 << 13
+    home = ws.get(rows, 8, 128, dev)[0].data_ptr()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        o = ws.get(rows, 8, 128, dev)[0]
+        torch.cuda._sleep(50_000_000)  # some tens of milliseconds
+        o.fill_(1.0)
+        del o
+        ws.get(4 * rows, 8, 128, dev)
+    other = torch.full((rows * 8 * 128,), 2.0, device=cuda)  # on the home stream, which does not wait
+    assert other.data_ptr() != home
+    torch.cuda.synchronize()
+    assert (other == 2).all()
