@@ -430,7 +430,7 @@ def _targets(t: OutTargets | None):
 
 FP4_ROWS = BLOCK_SIZE + 1  # rows of a (block, head): 16 tokens' codes, then their scales
 FP4_RUN = 32  # dims that share a scale
-WIDE_REDUCE_PIECES = 8  # rows of more pieces than this are reduced by a CTA per head instead of a warp
+WIDE_REDUCE_PIECES = 8  # few rows of more pieces than this are reduced by a CTA per head instead of a warp
 
 
 def is_fp4(pool: torch.Tensor) -> bool:
@@ -545,6 +545,16 @@ def kv_read_fp4(k_cache: torch.Tensor, v_cache: torch.Tensor, slot_mapping: torc
     return k, v
 
 
+def wide_reduction(plan: AttentionPlan) -> bool:
+    """Whether a step's split rows are reduced by a CTA per (token, head) (mlb_splitk_reduce_wide) or by a warp.  Both
+    launch over every token.  1000 CTAs cost 1.04 us, split or not; the warp's rows cost it 0.07 us a piece up to 32
+    pieces and 0.2 us a piece above, whatever their number (us, warp / CTA, 32 heads: one row of 63 pieces 13.2 / 3.6,
+    beside 255 others 13.2 / 9.3, 511 13.3 / 17.7, 8191 35 / 272; 16 rows of 30 4.2 / 3.6; 64 rows of 16 3.5 / 7.4;
+    4 of 9 2.25 / 2.19; 16 rows of 131072 tokens in 16, attention and all, 387 / 385)."""
+    pieces = plan.max_pieces
+    return pieces > WIDE_REDUCE_PIECES and plan.num_tokens * plan.num_heads <= pieces * (128 if pieces > 32 else 32)
+
+
 def attention_partials_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
                            seq_lens: torch.Tensor, qo_indptr: torch.Tensor, plan: AttentionPlan,
                            workspace: Workspace, out: torch.Tensor | None = None, scale: float | None = None,
@@ -612,8 +622,7 @@ def paged_attention_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     if plan.num_partial_rows and plan.num_tokens:
         dev = q.get_device()
         po, plse = workspace.get(plan.num_partial_rows, plan.num_heads, q.shape[2], q.device)
-        wide = plan.max_pieces > WIDE_REDUCE_PIECES
-        _launch(_lib.SPLITK_REDUCE_WIDE if wide else _lib.SPLITK_REDUCE, "splitk_reduce", dev, po.data_ptr(),
+        _launch(_lib.SPLITK_REDUCE_WIDE if wide_reduction(plan) else _lib.SPLITK_REDUCE, "splitk_reduce", dev, po.data_ptr(),
                 plse.data_ptr(), plan.num_partial_rows, plan.reduce_rows.data_ptr(), plan.reduce_chunks.data_ptr(),
                 plan.tokens_per_tile, plan.num_tokens, plan.num_heads, q.shape[2], _adr(out), *_strides(out),
                 DTYPE_CODE[q.dtype], 0 if targets is None else ctypes.addressof(targets))

@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import weakref
 
+import numpy as np
 import pytest
 import torch
 
@@ -65,3 +66,19 @@ def test_workspace_releases_what_it_keeps(mlb):
     assert all(r() is not None for r in first)
     ws.release()
     assert all(r() is None for r in first) and ws.get(5, 2, 64, dev)[0] is last[0]
+
+
+def test_reduction_goes_by_pieces_and_by_rows(mlb):
+    """A CTA per (token, head) is for few rows of many pieces: thousands of unsplit rows beside one long row would
+    launch a CTA each that has nothing to do."""
+
+    def plan(lens, new):  # with block tables, as the backend plans: long chunks become query tiles
+        tables = np.arange(len(lens) * 8192, dtype=np.int32).reshape(len(lens), 8192)
+        return mlb.plan_attention([sum(new[:i]) for i in range(len(new) + 1)], lens, 8192, 32, 8, "cpu",
+                                  pool_dtype=torch.uint8, block_tables_host=tables)
+
+    long_row, mixed = plan([32001], [1]), plan([32001, 8192], [1, 8192])
+    assert long_row.max_pieces > 32 and mixed.max_pieces > 32
+    assert mlb.ops.wide_reduction(long_row) and not mlb.ops.wide_reduction(mixed)
+    assert mlb.ops.wide_reduction(plan([131072] * 4, [1] * 4))
+    assert not mlb.ops.wide_reduction(plan([700] * 64, [1] * 64))

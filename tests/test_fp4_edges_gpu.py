@@ -138,3 +138,16 @@ def test_an_outgrown_buffer_waits_for_the_stream_that_uses_it(mlb, cuda):
     assert other.data_ptr() != home
     torch.cuda.synchronize()
     assert (other == 2).all()
+
+
+@pytest.mark.parametrize("first", [True, False])
+def test_one_long_row_beside_a_chunk(mlb, cuda, first):
+    """A row of many pieces among unsplit ones: each is reduced, or left alone, for itself."""
+    steps = [(9000, 1), (0, 600)] if first else [(0, 600), (9000, 1)]
+    st = Step(mlb, cuda, 8, 2, 64, steps, torch.bfloat16)
+    plan = st.plan(mlb, cuda)
+    assert plan.max_pieces > mlb.ops.WIDE_REDUCE_PIECES and not mlb.ops.wide_reduction(plan)
+    st.check(st.run(mlb, cuda))
+    alone = Step(mlb, cuda, 8, 2, 64, [(9000, 1)], torch.bfloat16)
+    assert mlb.ops.wide_reduction(alone.plan(mlb, cuda))
+    alone.check(alone.run(mlb, cuda))
