@@ -469,6 +469,16 @@ def _adr(t: torch.Tensor | None) -> int:
     return 0 if t is None else t.data_ptr()
 
 
+def _err_adr(err: torch.Tensor | None, device: int, what: str) -> int:
+    """Address of a device error word (int32, on the device of the launch), 0 for none."""
+    if err is None:
+        return 0
+    if err.dtype is not torch.int32 or err.get_device() != device or not err.numel():
+        raise ValueError(f"{what}: err must be an int32 tensor on the pools' device, got {err.dtype} "
+                         f"{tuple(err.shape)} on {err.device}")
+    return err.data_ptr()
+
+
 # A decode step makes several of these calls per layer, each a few microseconds on the GPU: every entry point below
 # tests its arguments with one expression of cheap attributes, and only where that fails with the checks that say what
 # is wrong (or that the case is an uncommon one that is fine: an empty tensor's strides).
@@ -520,7 +530,7 @@ def kv_append_fp4(k_cache: torch.Tensor, v_cache: torch.Tensor, slot_mapping: to
         _code(k, what)
     if shape[0]:
         _launch(_lib.KV_APPEND_FP4, what, dev, k_cache.data_ptr(), v_cache.data_ptr(), nb, slot_mapping.data_ptr(),
-                k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], code, shape[0], hkv, dh, _adr(err))
+                k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], code, shape[0], hkv, dh, _err_adr(err, dev, what))
 
 
 def kv_read_fp4(k_cache: torch.Tensor, v_cache: torch.Tensor, slot_mapping: torch.Tensor,
@@ -541,7 +551,7 @@ def kv_read_fp4(k_cache: torch.Tensor, v_cache: torch.Tensor, slot_mapping: torc
     v = torch.empty_like(k)
     if n:
         _launch(_lib.KV_READ_FP4, what, dev, k_cache.data_ptr(), v_cache.data_ptr(), nb, slot_mapping.data_ptr(),
-                k.data_ptr(), v.data_ptr(), DTYPE_CODE[dtype], n, hkv, dh, _adr(err))
+                k.data_ptr(), v.data_ptr(), DTYPE_CODE[dtype], n, hkv, dh, _err_adr(err, dev, what))
     return k, v
 
 
@@ -604,7 +614,7 @@ def attention_partials_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
             block_tables.stride(0), seq_lens.data_ptr(), qo_indptr.data_ptr(), seq_lens.shape[0], plan.units.data_ptr(),
             plan.num_units, plan.shared_units.data_ptr(), plan.num_shared_units, plan.members.data_ptr(), _adr(po),
             _adr(plse), plan.num_partial_rows, _adr(out), o0, o1, 0 if targets is None else ctypes.addressof(targets),
-            _adr(err))
+            _err_adr(err, dev, what))
     return out
 
 
@@ -731,7 +741,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, cos_
     rows, rot = cos_sin.shape
     _launch(_lib.QK_NORM_ROPE, what, dev, q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], code,
             n, h, hkv, dh, positions.data_ptr(), cos_sin.data_ptr(), rows, rot, _adr(q_weight), _adr(k_weight),
-            eps, qo.data_ptr(), qos[0], qos[1], ko.data_ptr(), kos[0], kos[1], _adr(err))
+            eps, qo.data_ptr(), qos[0], qos[1], ko.data_ptr(), kos[0], kos[1], _err_adr(err, dev, what))
     return qo, ko
 
 
@@ -763,7 +773,7 @@ def qk_norm_rope_append_fp4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, p
     _launch(_lib.QK_NORM_ROPE_APPEND_FP4, what, dev, q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1],
             v.data_ptr(), vs[0], vs[1], code, n, h, hkv, dh, positions.data_ptr(), cos_sin.data_ptr(), rows, rot,
             _adr(q_weight), _adr(k_weight), eps, out.data_ptr(), os[0], os[1], k_cache.data_ptr(), v_cache.data_ptr(), nb,
-            slot_mapping.data_ptr(), _adr(err))
+            slot_mapping.data_ptr(), _err_adr(err, dev, what))
     return out
 
 

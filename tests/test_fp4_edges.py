@@ -82,3 +82,14 @@ def test_reduction_goes_by_pieces_and_by_rows(mlb):
     assert mlb.ops.wide_reduction(long_row) and not mlb.ops.wide_reduction(mixed)
     assert mlb.ops.wide_reduction(plan([131072] * 4, [1] * 4))
     assert not mlb.ops.wide_reduction(plan([700] * 64, [1] * 64))
+
+
+def test_error_words_are_checked(mlb):
+    """Kernels write through the pointer: a tensor of another device or type must not get that far."""
+    word = mlb.ops._err_adr
+    assert word(None, 0, "x") == 0
+    good = torch.zeros(1, dtype=torch.int32)
+    assert word(good, -1, "x") == good.data_ptr()  # -1: the ordinal of CPU tensors
+    for bad, dev in ((good, 0), (good.long(), -1), (good.float(), -1), (good[:0], -1)):
+        with pytest.raises(ValueError, match="x: err"):
+            word(bad, dev, "x")

@@ -151,3 +151,24 @@ def test_one_long_row_beside_a_chunk(mlb, cuda, first):
     alone = Step(mlb, cuda, 8, 2, 64, [(9000, 1)], torch.bfloat16)
     assert mlb.ops.wide_reduction(alone.plan(mlb, cuda))
     alone.check(alone.run(mlb, cuda))
+
+
+def test_error_words_of_another_device_or_type_are_refused(mlb, cuda):
+    st = Step(mlb, cuda, 8, 2, 64, [(20, 1)], torch.bfloat16)
+    m, pools = st.meta, (st.k_pool, st.v_pool)
+    x, slots, table = torch.zeros(1, 2, 64, dtype=torch.bfloat16, device=cuda), m.slot_mapping, torch.ones(32, 64, device=cuda)
+    calls = (lambda e: mlb.kv_append_fp4(*pools, slots, x, x, err=e), lambda e: mlb.kv_read_fp4(*pools, slots, err=e),
+             lambda e: mlb.qk_norm_rope(x, x, m.positions, table, err=e),
+             lambda e: mlb.qk_norm_rope_append_fp4(x, x, x, m.positions, table, *pools, slots, err=e),
+             lambda e: st.run(mlb, cuda, err=e))
+    before = [p.clone() for p in pools]
+    for call in calls:
+        for bad in (torch.zeros(1, dtype=torch.int32), torch.zeros(1, dtype=torch.int64, device=cuda),
+                    torch.zeros(0, dtype=torch.int32, device=cuda)):
+            with pytest.raises(ValueError, match="err must be"):
+                call(bad)
+    assert all(torch.equal(a, b) for a, b in zip(pools, before))
+    for call in calls:
+        err = torch.zeros(1, dtype=torch.int32, device=cuda)
+        call(err)
+        assert int(err.item()) == 0
