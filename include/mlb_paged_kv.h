@@ -48,7 +48,8 @@ enum {
 /* Description of the last failing call on this thread ("" if none). */
 MLB_API const char* mlb_last_error(void);
 
-/* ABI version (bumped on any signature change). */
+/* ABI version: bumped when the signature or the meaning of an entry point changes.  Entry points may be added under
+ * one version (those of 4-bit pools and mlb_splitk_reduce_wide came under 10): look such a symbol up before its use. */
 MLB_API int mlb_abi_version(void);  /* 10 */
 
 /*
@@ -150,7 +151,7 @@ typedef struct {
  * Inputs: qo_indptr [num_seqs + 1] and seq_lens [num_seqs] exactly as AttentionMetadata holds them
  * (metadata.py:39-40, :97-98); max_blocks_per_seq = block_tables width (validates seq_lens).
  * block_tables_host (optional, may be NULL): a host copy of the int32 block tables with row stride
- * bt_stride_host; pass it for 16-bit pools only.  When given, decode rows whose tables start with the same
+ * bt_stride_host; pass it for 16- and 4-bit pools only.  When given, decode rows whose tables start with the same
  * run of block ids (shared prefix blocks) get shared-prefix units (a cascade split), and rows of >= 16 new
  * tokens get query-tile units (kind 1 above) instead of 8-column work units.  pages_per_unit = 0 picks a
  * split size from the total work and num_sms for 16- and 32-bit pools, MLB_PAGES_PER_UNIT_FP4 one for 4-bit pools.
@@ -452,7 +453,9 @@ MLB_API int mlb_qk_norm_rope_append_fp4(const void* q, int64_t q_stride_tok, int
  * mlb_paged_attention over 4-bit pools: q and out are fp16 or bf16, the plan is mlb_plan_attention's (units,
  * shared units and query tiles alike), partial rows are completed by mlb_splitk_reduce.  head_dim 64 / 128 / 256,
  * at most 8 query heads per KV head, scale positive and finite times log2(e).  Stored values enter the products exactly; P is rounded to
- * fp16, sums are fp32.
+ * fp16: 2^-11 relative for weights down to 2^-24 of a row's largest, 2^-35 of it absolute below.  bf16 query elements
+ * are exact down to 2^-31 of their row's largest.  Sums are fp32, so scores (times log2(e)) of 2^23 and more in
+ * magnitude are not resolved.
  */
 MLB_API int mlb_paged_attention_fp4(const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k_cache,
                       const void* v_cache, int dtype, int64_t num_blocks, int num_heads, int num_kv_heads,

@@ -101,7 +101,7 @@ class B200Backend(AttentionBackend):
     def plan(self, meta, num_heads: int, num_kv_heads: int, device: torch.device,
              dtype: torch.dtype = torch.bfloat16) -> AttentionPlan:
         """The step's plan, built on the first call with a new `meta` and reused after.  Shared-prefix units
-        and query tiles are planned from the host block tables (`host_fields`) when the pools are 16-bit."""
+        and query tiles are planned from the host block tables (`host_fields`) when the pools are 16- or 4-bit."""
         key = (num_heads, num_kv_heads, device, dtype)
         if self._planned is not meta or self._plan_key != key:
             tables = self.host_fields(meta)[0] if dtype != torch.float32 else None

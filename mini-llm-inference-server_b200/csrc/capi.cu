@@ -111,7 +111,9 @@ struct Group {
 // estimated step.  A CTA's time is its pages plus a start and an end worth kFp4CtaPages pages; up to 4 CTAs are
 // resident per SM, and one with fewer neighbours runs faster (measured on B200, rows of 8 KV heads: 64 CTAs of 256
 // pages 28.7 us, 128 of 128 18.3, 256 of 64 16.4, 512 of 128 38.4); a split costs the reduction's launch and its
-// rows.  Units of one length: what counts is the SM with the most of them (16 x 131072 tokens: 768 CTAs 444 us,
+// rows.  The constants are those of heads of 128 dims; other heads' plans are as right, and slower than they need be (a
+// page of 64 dims is half the work, and of 256 dims 2 CTAs are resident: 64 rows of 512..4096 tokens of 32 + 8 heads
+// 26, 41 and 83 us for 64, 128 and 256 dims, 1.7 to 2.2 times their bytes).  Units of one length: what counts is the SM with the most of them (16 x 131072 tokens: 768 CTAs 444 us,
 // 1152 405, 4096 395).  Of several lengths: 1 to 1.6 waves leave SMs idle at the end (64 rows of 512..4096 tokens:
 // 688 CTAs 43.5 us, 776 45.9, 1032 40.9, 1136 39.3; 4 KV heads: 568 24.9, 684 30.5).
 constexpr int kFp4CtasPerSm = 4;
@@ -373,7 +375,7 @@ int mlb_plan_attention(const int32_t* qo_indptr, const int32_t* seq_lens, int nu
   const int group_size = num_heads / num_kv_heads;
 
   // ---- multi-token rows (prefill chunks on cache) of >= kPrefillMinTokens tokens: with host tables
-  // (16-bit pools) they are planned as query tiles of 128 columns below instead of 8-column groups
+  // (16- and 4-bit pools) they are planned as query tiles of 128 columns below instead of 8-column groups
   std::vector<int> prefill_seqs;
   if (block_tables_host && bt_stride_host > 0) {
     std::vector<char> is_prefill(num_seqs, 0);

@@ -10,8 +10,9 @@
 // two runs of 8 dims, [8c, 8c + 8) and [r/2 + 8c, r/2 + 8c + 8): the two halves of its rotation pairs, so nothing
 // is exchanged but the sum of squares (log2(Dh / 16) shuffles) and, for the codes, the maximum over the 4 lanes of
 // a run of 32.  Loads and stores are 16 bytes a lane.  Heads of 128 dims: rotating 8192 tokens of 32 + 8 heads takes
-// 31 us, 5.5 TB/s, and 64 tokens with norms 2.4 us; appending 16384 tokens of 8 heads and reading them back 32 us,
-// 5.2 TB/s over both; norm, rotation and append of 4001 tokens of 28 + 4 heads 16 us.
+// 31 us, 5.5 TB/s (with norms 33), and 64 tokens with norms 2.3 us; appending 16384 tokens of 8 heads 17 us and reading
+// them back 15, 5.3 TB/s over both; norm, rotation and append of 4001 tokens of 28 + 4 heads 15 us (14 without norms).
+// fp32 rows, twice the bytes: 60, 38, 38 and 33 us; the append is then bound by quant_store_any's quotients.
 #include <algorithm>
 
 #include "fp4.cuh"

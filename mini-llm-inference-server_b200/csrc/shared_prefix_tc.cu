@@ -41,8 +41,9 @@
 // exact) and store them where TMA would have put them; rows that must not be seen (a bad block id, past the sequence's
 // end) are stored as zeros, so nothing is cleared later.  Q and P are fp16 for both output types: a bf16 query row is
 // divided by a power of two (fp4_query_scale), which goes into the row's softmax scale.
-// 4 chunks of 1500..2000 tokens on up to 8192 (32 + 8 heads of 128 dims): 589 us, 0.85 PFLOP/s (16-bit pools 703);
-// 128 rows behind a prefix of 512 blocks 51 us (16-bit pools 55).  What bounds it is the chain S -> softmax -> P of a
+// 4 chunks of 1500..2000 tokens on up to 8192 (32 + 8 heads of 128 dims): 590 us, 0.85 PFLOP/s (16-bit pools 708);
+// 128 rows behind a prefix of 512 blocks 56 us, no faster than 16-bit pools (56; one 4-bit set of inputs repeated stays
+// in L2: 52).  What bounds it is the chain S -> softmax -> P of a
 // query tile, not a unit (tensor pipe 41% busy, special functions 44%, issue slots 39%): a quarter of the exponentials
 // as polynomials on the FMA pipe made it 625 us, the maximum taken beside the exponentials 820.
 //

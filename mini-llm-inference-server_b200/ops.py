@@ -751,7 +751,8 @@ def qk_norm_rope_append_fp4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, p
                             k_weight: torch.Tensor | None = None, eps: float = 1e-6,
                             out: torch.Tensor | None = None, err: torch.Tensor | None = None) -> torch.Tensor:
     """`qk_norm_rope` and `kv_append_fp4` of its keys and of v in one launch: the cache and the returned queries are
-    bit-identical to the two calls'.  cos_sin must rotate the whole head (rot_dim == Dh)."""
+    bit-identical to the two calls'.  cos_sin must rotate the whole head (rot_dim == Dh).  out may be q, else memory
+    that overlaps none of the inputs.  A token whose position is outside the table is neither stored nor returned."""
     what = "qk_norm_rope_append_fp4"
     nb, hkv, dh = _check_fp4_pools(k_cache, v_cache, what)
     code, (n, h, q_dh), k_heads, dev, qs, ks = _check_rope(what, q, k, positions, cos_sin, q_weight, k_weight)
