@@ -238,7 +238,7 @@ class Workspace:
         """Free every outgrown buffer, once the GPU is done with them.  No graph that was captured with this workspace
         before may be replayed after."""
         for device, pairs in self._pairs.items():
-            if len(pairs) > 1 and device.type == "cuda":
+            if device.type == "cuda":
                 torch.cuda.synchronize(device)
             del pairs[:-1]
             for p in pairs:

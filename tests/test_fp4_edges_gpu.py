@@ -172,3 +172,22 @@ def test_error_words_of_another_device_or_type_are_refused(mlb, cuda):
         err = torch.zeros(1, dtype=torch.int32, device=cuda)
         call(err)
         assert int(err.item()) == 0
+
+
+def test_release_waits_for_streams_that_used_a_captured_buffer(mlb, cuda):
+    """A large buffer that a capture was given is not followed from stream to stream: release waits for all of them,
+    before the buffer in use can be outgrown and freed as any other."""
+    backend, dev = mlb.get_backend("b200"), torch.zeros(1, device=cuda).device
+    ws, rows = backend._workspace, 1 << 13
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ws.get(rows, 8, 128, dev)[0].fill_(0.0)
+    del g
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        o = ws.get(rows, 8, 128, dev)[0]
+        torch.cuda._sleep(50_000_000)  # some tens of milliseconds
+        o.fill_(1.0)
+    backend.release_scratch()
+    assert side.query()
